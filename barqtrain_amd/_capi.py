@@ -96,13 +96,23 @@ _SIGNATURES = {
                                       + [ctypes.c_float] + [c_i64] * 3 + [c_ptr, c_i64, c_ptr]),
 }
 
+RAGGED_HEADER = build.INCLUDE / "barq_ragged.h"
+_RAGGED_SIGNATURES = {
+    "barq_map_slots": (ctypes.c_int, [_POOL, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_i64] + [c_ptr] * 4),
+    "barq_write_slots": (ctypes.c_int, [_POOL, c_ptr, c_ptr, c_i64, c_ptr, c_ptr] + [c_i64] * 3 + [c_ptr]),
+    "barq_tree_attention": (ctypes.c_int, [_POOL, _COLD, c_ptr] + [c_i64] * 6 + [c_ptr, c_ptr] + [c_i64] * 3 + [c_ptr]
+                            + [c_i64] * 3 + [c_ptr] + [c_i64] * 3 + [ctypes.c_float] + [c_i64] * 3
+                            + [c_ptr, c_i64, c_ptr]),
+    "barq_tree_attention_workspace_bytes": (c_i64, [_POOL] + [c_i64] * 5),
+}
+
 _LIB: Optional[ctypes.CDLL] = None
 
 
 def header_functions(header: Path = HEADER) -> list[str]:
     """Names of the functions the header declares."""
     text = re.sub(r"/\*.*?\*/", "", header.read_text(), flags=re.S)
-    return sorted(set(re.findall(r"^\s*(?:const\s+)?\w+\s*\*?\s*(barq_kv_\w+)\s*\(", text, flags=re.M)))
+    return sorted(set(re.findall(r"^\s*(?:const\s+)?\w+\s*\*?\s*(barq_\w+)\s*\(", text, flags=re.M)))
 
 
 def load_library(path: Optional[Path] = None) -> ctypes.CDLL:
@@ -112,7 +122,7 @@ def load_library(path: Optional[Path] = None) -> ctypes.CDLL:
     import torch  # noqa: F401  -- share torch's HIP runtime
 
     lib = ctypes.CDLL(str(path or build.lib_path()))
-    for name, (res, args) in _SIGNATURES.items():
+    for name, (res, args) in {**_SIGNATURES, **_RAGGED_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

@@ -25,14 +25,14 @@ INCLUDE = REPO_ROOT / "include"
 LIB_NAME = "libbarq_kv.so"
 EXT_NAME = "barqtrain_cuda"
 OFFLOAD_ARCH = "gfx950"
-HIP_SOURCES = ("barq_kv.hip", "barq_kv_attention.hip", "barq_kv_quant.hip")
+HIP_SOURCES = ("barq_kv.hip", "barq_kv_attention.hip", "barq_kv_quant.hip", "barq_ragged.hip", "barq_tree.hip")
 HIP_HEADERS = ("fastdiv.h", "barq_kv_fp8.h", "barq_kv_commit.h", "barq_kv_internal.h")
 HOST_SOURCES = ("barq_kv_torch.cpp",)
 
 
 def source_files() -> tuple[Path, ...]:
     """Every file the build reads: the HIP sources and headers, the binding, the C ABI header."""
-    return tuple(CSRC / f for f in HIP_SOURCES + HIP_HEADERS + HOST_SOURCES) + (INCLUDE / "barq_kv.h",)
+    return tuple(CSRC / f for f in HIP_SOURCES + HIP_HEADERS + HOST_SOURCES) + (INCLUDE / "barq_kv.h", INCLUDE / "barq_ragged.h")
 
 # Packed fp32 instructions stay off in every HIP compile (none are needed: the kernels only
 # move bits, but the flag keeps the compiler from forming them).

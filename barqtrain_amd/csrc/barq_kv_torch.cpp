@@ -15,6 +15,7 @@
 
 #include "barq_kv.h"
 #include "barq_kv_internal.h"
+#include "barq_ragged.h"
 
 namespace {
 
@@ -843,6 +844,171 @@ void pool_decode_attention_cold(std::vector<at::Tensor> pool, std::vector<at::Te
   decode_attention_into(pool, &c, query, out, scale, max_seq, split_tokens, workspace);
 }
 
+// lengths[i] new tokens into row rows[i] (or i) of a group's pools, checked against the pools' host shadows
+// (lens, hws: updated in place; free_counts: at least so many pages are free): (slots, positions, requests,
+// offsets, pages taken of each pool), or None, nothing done, when the checked Python path must look at the call.
+py::object pool_map_slots_(const at::Tensor& group, const at::Tensor& pages, const c10::optional<std::vector<int64_t>>& rows,
+                           const std::vector<int64_t>& lengths, const std::vector<py::buffer>& lens,
+                           const std::vector<py::buffer>& hws, const std::vector<int64_t>& free_counts, int64_t limit,
+                           bool layers) {
+  int64_t num = 0;
+  const barq_kv_pool* pools = group_pools(group, &num);
+  const barq_kv_pool& g = pools[0];
+  TORCH_CHECK(pages.is_cuda() && pages.data_ptr() == g.key_pages, "pages do not belong to the group");
+  const int64_t n = (int64_t)lengths.size();
+  TORCH_CHECK((int64_t)lens.size() == num && (int64_t)hws.size() == num && (int64_t)free_counts.size() == num,
+              "pool_map_slots_: one shadow per pool");
+  if ((rows && (int64_t)rows->size() != n) || n > g.max_batch) return py::none();
+  limit = std::min(limit, g.max_blocks * g.page_size);
+  std::vector<int32_t> r32(n), n32(n);
+  int64_t total = 0;
+  for (int64_t i = 0; i < n; ++i) {
+    const int64_t r = rows ? (*rows)[i] : i;
+    if (r < 0 || r >= g.max_batch || lengths[i] < 0 || lengths[i] > limit) return py::none();
+    r32[i] = (int32_t)r;
+    n32[i] = (int32_t)lengths[i];
+    total += lengths[i];
+  }
+  if (total >= (int64_t(1) << 30)) return py::none();
+  if (rows) {
+    std::vector<bool> seen(g.max_batch);
+    for (const int32_t r : r32) {
+      if (seen[r]) return py::none();
+      seen[r] = true;
+    }
+  }
+  std::vector<int64_t*> L(num), W(num);
+  std::vector<int64_t> need(num, 0);
+  for (int64_t l = 0; l < num; ++l) {
+    const barq_kv_pool& p = pools[l];
+    if (p.max_batch != g.max_batch || p.max_blocks != g.max_blocks || p.page_size != g.page_size) return py::none();
+    L[l] = shadow(lens[l], g.max_batch);
+    W[l] = shadow(hws[l], g.max_batch);
+    for (int64_t m = 0; m < l; ++m)
+      if (L[m] == L[l]) return py::none();
+    for (int64_t i = 0; i < n; ++i) {
+      const int64_t r = r32[i], end = L[l][r] + n32[i];
+      if (L[l][r] != L[0][r] || (n32[i] > 0 && end > limit)) return py::none();
+      if (n32[i] > 0)
+        need[l] += std::max<int64_t>((end + p.page_size - 1) / p.page_size - (W[l][r] + p.page_size - 1) / p.page_size, 0);
+    }
+    if (need[l] > free_counts[l]) return py::none();
+  }
+  c10::DeviceGuard guard(pages.device());
+  const auto wide = pages.options().dtype(at::kLong), narrow = pages.options().dtype(at::kInt);
+  at::Tensor slots = layers ? at::empty({num, total}, wide) : at::empty({total}, wide);
+  at::Tensor both = at::empty({2, total}, narrow), offsets = at::empty({n + 1}, narrow);
+  if (n == 0) offsets.zero_();
+  check_status(barq_map_slots(pools, num, rows ? r32.data() : nullptr, n32.data(), n, slots.data_ptr<int64_t>(), total,
+                              both.data_ptr<int32_t>(), both.data_ptr<int32_t>() + total, offsets.data_ptr<int32_t>(),
+                              current_stream(pages)),
+               "pool_map_slots_");
+  for (int64_t l = 0; l < num; ++l)
+    for (int64_t i = 0; i < n; ++i) {
+      int64_t& len = L[l][r32[i]];
+      len += n32[i];
+      W[l][r32[i]] = std::max(W[l][r32[i]], len);
+    }
+  return py::make_tuple(slots, both[0], both[1], offsets, need);
+}
+
+// False, nothing done, when the checked Python path must look at the call.
+bool pool_write_slots_(const at::Tensor& handle, const at::Tensor& pages, const at::Tensor& slots, const at::Tensor& k,
+                       const at::Tensor& v, const c10::optional<at::Tensor>& index) {
+  const barq_kv_pool p = one_pool(handle, pages);
+  const auto flat = [&](const at::Tensor& t) {
+    return t.is_cuda() && t.get_device() == pages.get_device() && t.dim() == 1 && t.scalar_type() == at::kLong &&
+           t.is_contiguous();
+  };
+  if (!flat(slots) || (index && !(flat(*index) && index->numel() == slots.numel()))) return false;
+  if (k.dim() != 3 || k.size(1) != p.kv_heads || k.size(2) != p.head_dim || k.scalar_type() != pages.scalar_type() ||
+      v.scalar_type() != pages.scalar_type() || !k.is_cuda() || !v.is_cuda() || k.get_device() != pages.get_device() ||
+      v.get_device() != pages.get_device() || (k.size(2) > 1 && (k.stride(2) != 1 || v.stride(2) != 1)) ||
+      !same_layout(k, v) || k.size(0) < (index ? (int64_t)(slots.numel() > 0) : slots.numel()))
+    return false;
+  c10::DeviceGuard guard(pages.device());
+  check_status(barq_write_slots(&p, slots.data_ptr<int64_t>(), index ? index->data_ptr<int64_t>() : nullptr,
+                                slots.numel(), k.data_ptr(), v.data_ptr(), k.size(0), k.stride(0), k.stride(1),
+                                current_stream(pages)),
+               "pool_write_slots_");
+  return true;
+}
+
+// PagePool.attend_tree: the [batch, nodes, q_heads, head_dim] output (or `out`, [batch, q_heads, nodes, head_dim]),
+// or None when the checked Python path must look at the call.  max_seq < 0: the shadow's longest row, or in
+// a graph being recorded the capacity, since a replay's rows are the device's.  The workspace is the call's
+// own, from the allocator of its stream or graph: two graphs of one pool share none.
+c10::optional<at::Tensor> pool_attend_tree(const at::Tensor& handle, const c10::optional<at::Tensor>& cold,
+                                           const at::Tensor& pages, const at::Tensor& q, const at::Tensor& k,
+                                           const at::Tensor& v, const c10::optional<at::Tensor>& mask,
+                                           const c10::optional<at::Tensor>& out, py::buffer lens, double scale,
+                                           int64_t max_seq) {
+  const barq_kv_pool p = one_pool(handle, pages);
+  const auto dt = pages.scalar_type();
+  if ((dt != at::kBFloat16 && dt != at::kHalf) || q.dim() != 4 || k.dim() != 4) return c10::nullopt;
+  const int64_t batch = q.size(0), heads = q.size(1), nodes = q.size(2), device = pages.get_device();
+  const auto takes = [&](const at::Tensor& t) {
+    if (!t.is_cuda() || t.get_device() != device || t.scalar_type() != dt || t.stride(3) != 1 ||
+        (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) != 0)
+      return false;
+    for (int64_t d = 0; d < 3; ++d)
+      if (t.size(d) > 1 && t.stride(d) % 8 != 0) return false;
+    return true;
+  };
+  if (batch == 0 || heads == 0 || nodes == 0 || nodes > BARQ_TREE_MAX_NODES || batch > p.max_batch || q.size(3) != p.head_dim ||
+      heads % p.kv_heads != 0 || k.size(0) != batch || k.size(1) != p.kv_heads || k.size(2) != nodes ||
+      k.size(3) != p.head_dim || !takes(q) || !takes(k) || !takes(v) || !same_layout(k, v))
+    return c10::nullopt;
+  int64_t ms[3] = {0, 0, 0};
+  if (mask) {
+    const int64_t d = mask->dim();
+    if (!mask->is_cuda() || mask->get_device() != device || mask->scalar_type() != at::kBool || (d != 2 && d != 3) ||
+        mask->size(d - 2) != nodes || mask->size(d - 1) != nodes || (d == 3 && mask->size(0) != batch && mask->size(0) != 1))
+      return c10::nullopt;
+    ms[0] = d == 3 && mask->size(0) == batch && batch > 1 ? mask->stride(0) : 0;
+    ms[1] = mask->stride(d - 2);
+    ms[2] = mask->stride(d - 1);
+  }
+  c10::DeviceGuard guard(pages.device());
+  int64_t mean = 0;
+  if (max_seq < 0) {
+    if (recording(current_stream(pages))) {
+      max_seq = p.max_blocks * p.page_size;
+    } else {
+      const int64_t* L = shadow(lens, batch);
+      int64_t sum = 0;
+      max_seq = 1;
+      for (int64_t b = 0; b < batch; ++b) {
+        max_seq = std::max(max_seq, L[b]);
+        sum += L[b];
+      }
+      mean = std::max<int64_t>(sum / batch, 1);
+    }
+  }
+  max_seq = std::max<int64_t>(max_seq, 1);
+  const int64_t need = barq_tree_attention_workspace_bytes(&p, batch, heads, nodes, max_seq, mean);
+  if (need < 0) return c10::nullopt;
+  at::Tensor o = out ? *out : at::empty({batch, nodes, heads, p.head_dim}, q.options());
+  TORCH_CHECK(!out || (o.is_cuda() && o.get_device() == device && o.sizes() == q.sizes() &&
+                       (o.scalar_type() == dt || o.scalar_type() == at::kFloat)),
+              "out must match the query's shape, in the cache dtype or float32");
+  at::Tensor ws;
+  if (need > 0) ws = at::empty({need}, q.options().dtype(at::kByte));
+  const int64_t flags = (dt == at::kHalf ? BARQ_KV_ATTN_FP16 : 0) | (o.scalar_type() == at::kFloat ? BARQ_KV_ATTN_OUT_F32 : 0);
+  barq_kv_cold c;
+  if (cold) c = one_cold(*cold);
+  // a dimension of one has no stride that enters an address
+  const auto st = [](const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; };
+  const int64_t oh = out ? 1 : 2, on = out ? 2 : 1;
+  check_status(barq_tree_attention(&p, cold ? &c : nullptr, q.data_ptr(), batch, heads, nodes, st(q, 0), st(q, 1), st(q, 2),
+                                   k.data_ptr(), v.data_ptr(), st(k, 0), st(k, 1), st(k, 2),
+                                   mask ? (const uint8_t*)mask->data_ptr() : nullptr, ms[0], ms[1], ms[2], o.data_ptr(),
+                                   st(o, 0), st(o, oh), st(o, on), (float)scale, max_seq, mean, flags,
+                                   need > 0 ? ws.data_ptr() : nullptr, need, current_stream(pages)),
+               "pool_attend_tree");
+  return o;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -875,6 +1041,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cold_group", &cold_group, "Pack a pool's cold store for pool_step_cold_ and pool_attend");
   m.def("pool_step_cold_", &pool_step_cold_, "pool_step_ for a pool with a cold store (see QuantPagePool.update)");
   m.def("pool_attend", &pool_attend, "Decode attention with its host planning (see PagePool.attend)");
+  m.def("pool_map_slots_", &pool_map_slots_, "Block tables and slots of ragged requests (see paged.map_slots_layers)");
+  m.def("pool_write_slots_", &pool_write_slots_, "Store packed tokens through a slot map (see PagePool.write_slots)");
+  m.def("pool_attend_tree", &pool_attend_tree, "Attention of a drafted tree over a page pool (see PagePool.attend_tree)");
   m.def("select_workspace_words", &select_workspace_words, "Workspace words of pool_group_select_rows_");
   m.def("pool_group_select_rows_", &pool_group_select_rows_,
         "One row selection applied to every pool of a group, sharing full pages");

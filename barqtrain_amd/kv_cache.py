@@ -33,7 +33,9 @@ from barqtrain_amd.paged import (
     PagedKVPoolExhausted,
     PagePool,
     QuantPagePool,
+    SlotMap,
     crop_layers,
+    map_slots_layers,
     reset_layers,
     select_rows_layers,
 )
@@ -239,6 +241,17 @@ class BarqPagedKVCacheLayer(CacheLayerMixin):
         if self.is_initialized:
             self.pool.free_rows(rows)
 
+    def write_slots(self, slots: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                    index: Optional[torch.Tensor] = None) -> None:
+        """Store packed tokens, or the accepted nodes of drafted trees, in slots of this layer
+        (PagePool.write_slots; the slots come from the cache's map_slots)."""
+        self.pool.write_slots(slots, key, value, index)
+
+    def attend_tree(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                    mask: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+        """Attention of drafted tokens over this layer's rows and over one another (PagePool.attend_tree)."""
+        return self.pool.attend_tree(query, key, value, mask, scale)
+
     def offload(self):
         if self.is_initialized:
             self.pool.to("cpu")
@@ -306,6 +319,19 @@ class BarqPagedKVCache(Cache):
     def free_rows(self, rows) -> None:
         for layer in self.layers:
             layer.free_rows(rows)
+
+    def map_slots(self, lengths, rows=None) -> SlotMap:
+        """Take lengths[i] new tokens into row rows[i] of every layer (paged.map_slots_layers): block tables and
+        slots [layers, total] of the packed tokens, which each layer's write_slots stores.  The layers must be
+        initialised (have taken a first update, or lazy_initialization)."""
+        layers = self.layers
+        if not layers or not all(l.is_initialized for l in layers):
+            raise ValueError("map_slots: the cache's layers hold no pages yet")
+        got = map_slots_layers([l.pool for l in layers], lengths, rows, layers[0].max_cache_len)
+        last = 1 + max(range(len(lengths)) if rows is None else [int(r) for r in rows], default=-1)
+        for l in layers:
+            l.current_batch_size = max(l.current_batch_size, last)
+        return got
 
     # Cache.crop and Cache.reset, layer by layer in transformers: one launch for every layer's pool.
     def _pools(self):

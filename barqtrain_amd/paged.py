@@ -24,7 +24,7 @@ algorithm (same page-allocation order) written with torch CPU operators.
 from __future__ import annotations
 
 import math
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
 import torch
@@ -39,6 +39,7 @@ ERRBIT_BAD_INDEX = 4
 ERRBIT_OUT_SHORT = 8
 ERRBIT_ATTN_SHORT = 16
 SEQ_FROM_DEVICE = 1
+TREE_MAX_NODES = 256  # BARQ_TREE_MAX_NODES of include/barq_ragged.h
 NO_COMPRESS = 4  # BARQ_KV_NO_COMPRESS: an update of a quantised pool skips its compress launch
 SEPARATE_FINALIZE = 2
 
@@ -53,6 +54,15 @@ class PagedKVCapacityError(ValueError, RuntimeError):
 
 class PagedKVPoolExhausted(PagedKVCapacityError):
     """The pool has fewer free pages than an append needs."""
+
+
+class SlotMap(NamedTuple):
+    """Where a packed batch's tokens lie (PagePool.map_slots): token j of request i is number offsets[i] + j."""
+
+    slots: torch.Tensor      # int64 [total], or [layers, total]: page * page_size + place in the page
+    positions: torch.Tensor  # int32 [total]: position in the token's row
+    requests: torch.Tensor   # int32 [total]
+    offsets: torch.Tensor    # int32 [requests + 1]
 
 
 _KV_CACHE = None  # the kv_cache module, which imports this one
@@ -347,6 +357,52 @@ class PagePool:
         self.hw[r] = np.maximum(self.hw[r], self.lens[r])
         self.free_count -= need
 
+    def map_slots(self, lengths: Sequence[int], rows: Optional[Sequence[int]] = None,
+                  max_length: Optional[int] = None) -> SlotMap:
+        """Take ``lengths[i]`` new tokens into row ``rows[i]`` (default: row i; distinct rows): the pages they
+        need are mapped and the rows' lengths advanced as by an append, on the device, and the places of the
+        packed tokens returned, for `write_slots` or a kernel of the program's own to store them before the
+        rows are read.  Lengths are host numbers; 0 leaves a row as it is.  Nothing changes if a row would
+        pass `max_length` (default: its capacity) or the pool has too few pages."""
+        return _map_slots([self], lengths, rows, max_length, False)
+
+    def write_slots(self, slots: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                    index: Optional[torch.Tensor] = None) -> None:
+        """Store token ``index[j]`` (default: j) of ``key`` / ``value`` ``[tokens, kv_heads, head_dim]`` in slot
+        ``slots[j]`` (int64, as `map_slots` gives them; negative ones are passed over).  The accepted nodes of
+        drafted trees ``[batch, kv_heads, nodes, head_dim]`` are ``states.transpose(1, 2).flatten(0, 1)`` with
+        ``index`` = row * nodes + node."""
+        if self.on_gpu:
+            backend = _gpu_backend()
+            handle = self._packed()
+            if backend.pool_write_slots_(handle[1], self.key_pages, slots, key, value, index):
+                return
+        self._check_write(slots, key, value, index)
+        if slots.numel() == 0:
+            return
+        k, v = self._compatible_pair(key, value)
+        if not self.on_gpu:
+            _HostOps.pool_write_slots_(self.tensors, slots, k, v, index)
+            return
+        if not backend.pool_write_slots_(handle[1], self.key_pages, slots.contiguous(), k, v,
+                                         None if index is None else index.contiguous()):
+            raise RuntimeError("write_slots: the kernel does not take these tensors")
+
+    def _check_write(self, slots, key, value, index) -> None:
+        if key.dim() != 3 or key.shape != value.shape or tuple(key.shape[1:]) != (self.kv_heads, self.head_dim):
+            raise ValueError("write_slots: key and value must be [tokens, kv_heads, head_dim] alike, with the cache's heads")
+        if key.dtype != self.dtype or value.dtype != self.dtype:
+            raise ValueError("write_slots: key and value must have the cache dtype")
+        for name, t in (("slots", slots), ("index", index)):
+            if t is not None and (t.dim() != 1 or t.dtype != torch.int64):
+                raise ValueError(f"write_slots: {name} must be a flat int64 tensor")
+        if index is not None and index.numel() != slots.numel():
+            raise ValueError("write_slots: one index per slot")
+        if key.shape[0] < (slots.numel() if index is None else min(slots.numel(), 1)):
+            raise ValueError("write_slots: fewer tokens than slots")
+        if any(t is not None and t.device != self.key_pages.device for t in (slots, key, value, index)):
+            raise ValueError("write_slots: tensors must be on the cache device")
+
     def _new_out(self, batch: int, seq: int) -> tuple[torch.Tensor, torch.Tensor]:
         shape = (batch, self.kv_heads, seq, self.head_dim)
         return (torch.empty(shape, dtype=self.dtype, device=self.device),
@@ -566,6 +622,88 @@ class PagePool:
 
     def _attention_call(self, backend, query, out, scale, max_seq, split_tokens, ws):
         backend.pool_decode_attention(self.tensors, query, out, scale, max_seq, split_tokens, ws)
+
+    def attend_tree(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                    mask: Optional[torch.Tensor] = None, scale: Optional[float] = None, *,
+                    out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                    max_seq: Optional[int] = None) -> torch.Tensor:
+        """Attention of drafted tokens -- the nodes of a tree -- over rows [0, batch) and over the tree itself.
+        `query` ``[batch, q_heads, nodes, head_dim]`` and `key` / `value` ``[batch, kv_heads, nodes, head_dim]``
+        are the nodes' own, which are not in the cache.  Node i sees its row's seq_lens[b] cached positions and
+        the nodes j with ``mask[b, i, j]`` (bool ``[nodes, nodes]`` or ``[batch, nodes, nodes]``; None: a chain,
+        node i sees nodes 0 .. i).  A node that sees nothing gives zeros; what a node does not see takes no
+        part, whatever it holds.  Nothing is stored: the accepted nodes go into the cache by `map_slots` and
+        `write_slots`.  Returns ``[batch, q_heads, nodes, head_dim]`` (a view of a ``[batch, nodes, q_heads,
+        head_dim]`` buffer) in `out_dtype` (default the query's).  `max_seq` bounds the rows' lengths
+        (default: the host shadow's longest row; in a graph being captured the capacity)."""
+        if self.on_gpu and out is None and out_dtype is None and max_seq is None:
+            got = self._attend_tree(query, key, value, mask, scale, None, -1)
+            if got is not None:
+                return got.transpose(1, 2)
+        self._check_tree(query, key, value, mask)
+        batch, q_heads, nodes, _ = query.shape
+        dt = out_dtype or (query.dtype if out is None else out.dtype)
+        if out is None:
+            out = torch.empty((batch, nodes, q_heads, self.head_dim), dtype=dt, device=query.device).transpose(1, 2)
+        elif out.shape != query.shape or out.dtype != dt or out.device != query.device:
+            raise ValueError("out must have the query's shape and device, and out_dtype")
+        if dt not in (self.dtype, torch.float32):
+            raise ValueError("attend_tree gives the pool's dtype or float32")
+        if max_seq is None:
+            max_seq = -1
+        elif not 0 <= max_seq <= self.capacity:
+            raise ValueError("max_seq exceeds the cache capacity")
+        if query.numel() == 0:
+            return out
+        if not self.on_gpu:
+            longest = int(self.lens[:batch].max()) if max_seq < 0 else int(max_seq)
+            ko, vo = self.gather(batch, longest)
+            _HostOps.attend_tree_over(ko, vo, np.minimum(self.lens, longest), query, key, value, mask, out,
+                                      1.0 / math.sqrt(self.head_dim) if scale is None else float(scale))
+            return out
+        aligned = lambda t: (t.stride(-1) == 1 and t.data_ptr() % 16 == 0  # noqa: E731
+                             and all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:3], t.stride()[:3])))
+        query = query if aligned(query) else _packed_copy(query)
+        key, value = self._compatible_pair(key, value)
+        if not (aligned(key) and aligned(value)):
+            key, value = _packed_copy(key), _packed_copy(value)
+        size = out.element_size()
+        if (out.stride(-1) != 1 or out.data_ptr() % (4 * size)
+                or any(n > 1 and s % 4 for n, s in zip(out.shape[:3], out.stride()[:3]))):
+            return out.copy_(self.attend_tree(query, key, value, mask, scale, out_dtype=dt,
+                                              max_seq=None if max_seq < 0 else max_seq))
+        if self._attend_tree(query, key, value, mask, scale, out, max_seq) is None:
+            raise RuntimeError("attend_tree: the kernel does not take these tensors")
+        return out
+
+    def _attend_tree(self, query, key, value, mask, scale, out, max_seq):
+        """attend_tree planned in the binding: ``[batch, nodes, q_heads, head_dim]`` (or `out`), or None when
+        `attend_tree` has to look at the call."""
+        scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
+        handle = self._packed()
+        return handle[3].pool_attend_tree(handle[1], handle[2], self.key_pages, query, key, value, mask, out,
+                                          self.lens, scale, max_seq)
+
+    def _check_tree(self, query, key, value, mask) -> None:
+        if self.on_gpu and (self.dtype not in (torch.bfloat16, torch.float16) or self.head_dim not in (64, 128, 256)):
+            raise ValueError("attend_tree takes bf16/fp16 pools with head_dim 64, 128 or 256 "
+                             f"(got {self.dtype}, head_dim {self.head_dim})")
+        if query.dim() != 4 or query.shape[3] != self.head_dim or query.shape[1] % self.kv_heads:
+            raise ValueError("query must be [batch, q_heads, nodes, head_dim] with q_heads a multiple of the pool's kv_heads")
+        batch, _, nodes, _ = query.shape
+        if batch > self.max_batch:
+            raise ValueError("query batch exceeds the pool's rows")
+        if nodes > TREE_MAX_NODES:
+            raise ValueError(f"a tree has at most {TREE_MAX_NODES} nodes (got {nodes})")
+        if tuple(key.shape) != (batch, self.kv_heads, nodes, self.head_dim) or value.shape != key.shape:
+            raise ValueError("key and value must be [batch, kv_heads, nodes, head_dim] of the query's nodes")
+        if any(t.dtype != self.dtype or t.device != self.key_pages.device for t in (query, key, value)):
+            raise ValueError("query, key and value must have the pool's dtype and device")
+        if mask is not None:
+            if mask.dtype != torch.bool or mask.device != query.device:
+                raise ValueError("the tree's mask must be bool, on the pool's device")
+            if tuple(mask.shape) not in ((nodes, nodes), (1, nodes, nodes), (batch, nodes, nodes)):
+                raise ValueError("the tree's mask must be [nodes, nodes] or [batch, nodes, nodes]")
 
     def attention_workspace(self, nbytes: int) -> torch.Tensor:
         """The pool's decode-attention workspace (split records), at least `nbytes`; grown, never
@@ -1044,6 +1182,35 @@ class QuantPagePool(PagePool):
             dst.select_rows(src_rows)
         return dst
 
+    def _attend_tree(self, query, key, value, mask, scale, out, max_seq):
+        if self.page_size % 16 == 0 and self.head_dim in (64, 128):
+            return super()._attend_tree(query, key, value, mask, scale, out, max_seq)
+        # Pages that the kernel does not decode: it reads the dequantising gather instead, each row as one page.
+        self._check_tree(query, key, value, mask)
+        batch = query.shape[0]
+        if query.numel() == 0:
+            return None
+        if max_seq < 0:
+            max_seq = self.capacity if self._recording() else self.max_len(batch)
+        seq = max(max_seq, 1)
+        both = torch.empty((2, batch, seq, self.kv_heads, self.head_dim), dtype=self.dtype, device=self.device)
+        self.gather(batch, seq, (both[0].transpose(1, 2), both[1].transpose(1, 2)))
+        table = torch.arange(batch, dtype=torch.int32, device=self.device).reshape(batch, 1)
+        spare = torch.zeros(2 * batch, dtype=torch.int32, device=self.device)
+        backend = _gpu_backend()
+        handle = backend.pool_group([[both[0], both[1], table, self.seq_lens[:batch], self.high_water[:batch],
+                                      spare[:batch], self.ctrl, spare[batch:]]])
+        return backend.pool_attend_tree(handle, None, both[0], query, key, value, mask, out, self.lens,
+                                        1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), seq)
+
+    def _settle(self) -> None:
+        """Quantise the blocks that `map_slots` left behind the window (written by now)."""
+        frontier, moved = self._cold_after(self.max_batch, 0)
+        if moved or self._recording():
+            self._ops().pool_compress_(self.tensors, self.cold_tensors, self.window, self.max_batch,
+                                       not self._recording())
+            self._quantised(self.max_batch, frontier, moved)
+
     def _attention_call(self, backend, query, out, scale, max_seq, split_tokens, ws):
         if self.page_size % 16 == 0 and self.head_dim in (64, 128):
             backend.pool_decode_attention_cold(self.tensors, self.cold_tensors, self.window, query, out, scale,
@@ -1165,6 +1332,100 @@ def select_rows_layers(pools: Sequence[PagePool], src_rows: Sequence[int]) -> No
     new_lens[:, :n], new_hw[:, :n] = lens[:, r], hw[:, r]
     for l, (p, k) in enumerate(zip(pools, need.tolist())):
         p._selected(new_lens[l], new_hw[l], int(k))
+
+
+def _packed_copy(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous copy at an aligned address (contiguous() returns a contiguous view as it is)."""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _host_ints(values, what: str) -> list[int]:
+    if isinstance(values, torch.Tensor) and values.device.type != "cpu":
+        raise ValueError(f"map_slots: {what} are host numbers (a device tensor would be read with a synchronisation)")
+    values = values.tolist() if hasattr(values, "tolist") else [int(v) for v in values]
+    if any(not isinstance(v, int) for v in values):
+        raise ValueError(f"map_slots: {what} must be a flat sequence of whole numbers")
+    return values
+
+
+def map_slots_layers(pools: Sequence[PagePool], lengths: Sequence[int], rows: Optional[Sequence[int]] = None,
+                     max_length: Optional[int] = None) -> SlotMap:
+    """``PagePool.map_slots`` on every pool of a model's layers (distinct pools of one device and geometry
+    whose rows have equal lengths), in one launch for each 256 requests of 32 layers; every pool is checked for
+    room before any changes.  ``slots`` is ``[layers, total]``; positions, requests and offsets are one for all."""
+    return _map_slots(list(pools), lengths, rows, max_length, True)
+
+
+def _map_slots(pools: list, lengths, rows, max_length: Optional[int], layers: bool, retried: bool = False) -> SlotMap:
+    if not pools:
+        raise ValueError("map_slots: no pools")
+    lengths = _host_ints(lengths, "lengths")
+    rows = None if rows is None else _host_ints(rows, "rows")
+    g = pools[0]
+    if any(getattr(p, "quantized", False) for p in pools):
+        _check_map(pools, lengths, rows, max_length, False)
+        for p in pools:
+            if getattr(p, "quantized", False):
+                p._settle()
+    if g.on_gpu and all(p.device == g.device for p in pools):
+        handle = g._packed() if len(pools) == 1 else (0, _pool_group(pools)["group"], None, _gpu_backend())
+        limit = g.capacity if max_length is None else int(max_length)
+        got = handle[3].pool_map_slots_(handle[1], g.key_pages, rows, lengths, [p.lens for p in pools],
+                                        [p.hw for p in pools], [p.free_count for p in pools], limit, layers)
+        if got is not None:
+            for p, need in zip(pools, got[4]):
+                p.free_count -= need
+            return SlotMap(*got[:4])
+    need = _check_map(pools, lengths, rows, max_length)
+    if g.on_gpu:  # only a lower bound of the free pages stood in the way, and is exact now
+        if retried:
+            raise RuntimeError("map_slots: the binding does not take this call")
+        return _map_slots(pools, lengths, rows, max_length, layers, True)
+    at = np.asarray(range(len(lengths)) if rows is None else rows, dtype=np.int64)
+    maps = [_HostOps.pool_map_slots_(p.tensors, at, lengths) for p in pools]
+    for p, k in zip(pools, need):
+        p.lens[at] += np.asarray(lengths, dtype=np.int64)
+        p.hw[at] = np.maximum(p.hw[at], p.lens[at])
+        p.free_count -= k
+    return maps[0] if not layers else maps[0]._replace(slots=torch.stack([m.slots for m in maps]))
+
+
+def _check_map(pools: list, lengths: list[int], rows: Optional[list[int]], max_length: Optional[int],
+               pages: bool = True) -> list[int]:
+    """Raise what stands against a map_slots call (with `pages`, too few free ones too); the pages that each
+    pool gives up for it."""
+    g = pools[0]
+    counts = np.asarray(lengths, dtype=np.int64)
+    at = np.asarray(range(len(lengths)) if rows is None else rows, dtype=np.int64)
+    if len(at) != len(lengths):
+        raise ValueError("map_slots: one row per length")
+    if len(at) and (at.min() < 0 or at.max() >= g.max_batch):
+        raise IndexError("map_slots: row out of range")
+    if len(np.unique(at)) != len(at):
+        raise ValueError("map_slots: rows must be distinct")
+    if any(n < 0 for n in lengths):
+        raise ValueError("map_slots: lengths must not be negative")
+    if sum(lengths) >= 1 << 30:
+        raise ValueError("map_slots: too many tokens for one call")
+    if len({id(p) for p in pools}) != len(pools):
+        raise ValueError("map_slots: a pool is named twice")
+    if any((p.device, p.max_batch, p.max_blocks, p.page_size) != (g.device, g.max_batch, g.max_blocks, g.page_size)
+           for p in pools):
+        raise ValueError("map_slots: the pools of one call must share device, rows, blocks and page size")
+    if any((p.lens[at] != g.lens[at]).any() for p in pools):
+        raise ValueError("map_slots: the layers' rows have different lengths; map each pool by itself")
+    ends = g.lens[at] + counts
+    limit = min(g.capacity, g.capacity if max_length is None else int(max_length))
+    worst = int(ends[counts > 0].max(initial=0))
+    if worst > limit and (counts > 0).any():
+        raise PagedKVCapacityError(f"paged KV cache capacity exceeded: requested {worst}, max_cache_len={limit}")
+    need = []
+    for p in pools:
+        new = -(-ends // p.page_size) - (-(-p.hw[at] // p.page_size))
+        need.append(int(np.maximum(np.where(counts > 0, new, 0), 0).sum()))
+        if pages:
+            p.ensure_free(need[-1], "map_slots")
+    return need
 
 
 def _one_device(pools: list) -> bool:
@@ -1335,6 +1596,54 @@ class _HostOps:
             s = s.masked_fill(pos > limit, float("-inf"))
             p = torch.softmax(s, dim=-1).nan_to_num(0.0)  # a row that sees nothing gives zeros
             out[b] = torch.matmul(p, v).to(out.dtype)
+
+    @staticmethod
+    def pool_map_slots_(t, rows, lengths):
+        kp, vp, bt, lens, hw, free, ctrl, shares = t
+        P, MB = _HostOps._geometry(t)
+        slots, positions, requests = [], [], []
+        for i, (r, n) in enumerate(zip(rows.tolist(), lengths)):
+            one = t[:2] + [bt[r:r + 1], lens[r:r + 1], hw[r:r + 1]] + t[5:]
+            pos = int(lens[r]) + torch.arange(n, dtype=torch.int64)
+            if n:
+                _HostOps._map_new_blocks(one, 1, n)
+                _HostOps._commit(one, 1, n)
+            page = bt[r, pos // P].long()
+            slots.append(torch.where(page < 0, page, page * P + pos % P))
+            positions.append(pos.int())
+            requests.append(torch.full((n,), i, dtype=torch.int32))
+        offsets = torch.tensor(np.concatenate([[0], np.cumsum(lengths)]), dtype=torch.int32)
+        join = lambda parts, dtype: torch.cat(parts) if parts else torch.empty(0, dtype=dtype)  # noqa: E731
+        return SlotMap(join(slots, torch.int64), join(positions, torch.int32), join(requests, torch.int32), offsets)
+
+    @staticmethod
+    def pool_write_slots_(t, slots, key, value, index):
+        kp, vp, ctrl = t[0], t[1], t[6]
+        src = torch.arange(slots.numel()) if index is None else index
+        named = slots >= 0
+        ok = named & (slots < kp.shape[0] * kp.shape[1]) & (src >= 0) & (src < key.shape[0])
+        if bool((named & ~ok).any()):
+            ctrl[CTRL_ERRORS] |= ERRBIT_BAD_INDEX
+        kp.flatten(0, 1)[slots[ok]] = key[src[ok]]
+        vp.flatten(0, 1)[slots[ok]] = value[src[ok]]
+
+    @staticmethod
+    def attend_tree_over(ko, vo, lens, query, key, value, mask, out, scale):
+        """attend_tree over gathered rows ko / vo ``[batch, kv_heads, seq, D]``, float32; what no node sees
+        takes no part, whatever it holds."""
+        B, q_heads, T, D = query.shape
+        group = q_heads // ko.shape[1]
+        mask = torch.ones((T, T), dtype=torch.bool).tril() if mask is None else mask
+        for b in range(B):
+            n = int(lens[b])
+            k = torch.cat([ko[b, :, :n], key[b]], dim=1).float().repeat_interleave(group, dim=0)
+            v = torch.cat([vo[b, :, :n], value[b]], dim=1).float().repeat_interleave(group, dim=0)
+            seen = torch.cat([torch.ones((T, n), dtype=torch.bool), mask.expand(B, T, T)[b]], dim=1)
+            s = torch.matmul(query[b].float(), k.transpose(1, 2)) * scale
+            p = torch.softmax(s.masked_fill(~seen, float("-inf")), dim=-1)
+            for i in range(T):  # a node's own positions only: 0 * NaN is not 0
+                x = torch.matmul(p[:, i:i + 1, seen[i]], v[:, seen[i]])[:, 0]
+                out[b, :, i] = x.to(out.dtype) if bool(seen[i].any()) else 0
 
     # -------------------------------------------------------------- fp8 cold store (host memory)
     @staticmethod
