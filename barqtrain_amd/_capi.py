@@ -103,7 +103,7 @@ _RAGGED_SIGNATURES = {
     "barq_tree_attention": (ctypes.c_int, [_POOL, _COLD, c_ptr] + [c_i64] * 6 + [c_ptr, c_ptr] + [c_i64] * 3 + [c_ptr]
                             + [c_i64] * 3 + [c_ptr] + [c_i64] * 3 + [ctypes.c_float] + [c_i64] * 3
                             + [c_ptr, c_i64, c_ptr]),
-    "barq_tree_attention_workspace_bytes": (c_i64, [_POOL] + [c_i64] * 5),
+    "barq_tree_attention_workspace_bytes": (c_i64, [_POOL] + [c_i64] * 6),
 }
 
 _LIB: Optional[ctypes.CDLL] = None

@@ -986,7 +986,7 @@ c10::optional<at::Tensor> pool_attend_tree(const at::Tensor& handle, const c10::
     }
   }
   max_seq = std::max<int64_t>(max_seq, 1);
-  const int64_t need = barq_tree_attention_workspace_bytes(&p, batch, heads, nodes, max_seq, mean);
+  const int64_t need = barq_tree_attention_workspace_bytes(&p, cold.has_value(), batch, heads, nodes, max_seq, mean);
   if (need < 0) return c10::nullopt;
   at::Tensor o = out ? *out : at::empty({batch, nodes, heads, p.head_dim}, q.options());
   TORCH_CHECK(!out || (o.is_cuda() && o.get_device() == device && o.sizes() == q.sizes() &&

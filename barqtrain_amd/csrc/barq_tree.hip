@@ -26,8 +26,10 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "barq_kv.h"
+#include "barq_kv_commit.h"
 #include "barq_kv_fp8.h"
 #include "barq_ragged.h"
 #include "fastdiv.h"
@@ -78,6 +80,7 @@ struct TreeArgs {
   int32_t units;             // pairs * splits
   int32_t pairs;
   float scale_log2;
+  int32_t batch, groups;     // of the flat schedule: rows, groups of workgroups
   // fp8 cold store: a table entry -2 - c names cold page c
   const uint8_t* kcodes;
   const uint8_t* vcodes;
@@ -562,14 +565,647 @@ __global__ void __launch_bounds__(kThreads) tree_join_kernel(const TreeArgs a, i
                   sum * by);
 }
 
+// ------------------------------------------------------------------- two-byte pages, asynchronous tiles
+// The flat schedule: every (row, KV head) pair's tiles, the tree's nodes first and then the cached positions, form
+// one list; group g of row_blocks workgroups takes the g-th equal range of it, whatever the rows' lengths.
+// A range's piece of a pair that is not the whole pair leaves a record (slot 2g for a piece that begins inside its
+// pair, else 2g + 1: a range has at most one of each), joined by a second launch in the order of the groups.
+template <int HD>
+struct Ring {
+  static constexpr int kTile = HD == 256 ? 32 : 64;  // positions of a tile
+  static constexpr int kBytes = kTile * HD * 2;      // of its keys, or values
+  static constexpr int kStages = 65536 / kBytes;     // tiles in LDS: 128 KB of them
+  static constexpr int kChunks = HD / 8;
+  static constexpr int kGroup = 64 / kChunks;        // positions that one load of a wave covers
+};
+
+__device__ __forceinline__ int row_length(const TreeArgs& a, int b) { return max(min(a.seq_lens[b], a.max_seq), 0); }
+
+template <int KT>
+__device__ __forceinline__ int pair_tiles(const TreeArgs& a, int len) {
+  return (len + KT - 1) / KT + (a.nodes + KT - 1) / KT;
+}
+
+// The list's length of one KV head's pair of row b: its tiles, after kPairCost places for what a pair costs besides.
+constexpr int kPairCost = 2;
+template <int KT>
+__device__ __forceinline__ int pair_places(const TreeArgs& a, int len) {
+  return pair_tiles<KT>(a, len) + kPairCost;
+}
+
+// Places of one KV head of rows [0, b), and of all rows.  Run by a whole wave.
+template <int KT>
+__device__ __forceinline__ void count_places(const TreeArgs& a, int b, int lane, int* before, int* all) {
+  int upto = 0, sum = 0;
+  for (int r0 = 0; r0 < a.batch; r0 += 64) {
+    const int r = r0 + lane;
+    const int t = r < a.batch ? pair_places<KT>(a, row_length(a, r)) : 0;
+    sum += barq_commit::wave_sum(t);
+    upto += barq_commit::wave_sum(r < b ? t : 0);
+  }
+  *before = upto;
+  *all = sum;
+}
+
+__device__ __forceinline__ int range_of(const TreeArgs& a, int all) {
+  return max(1, (all * a.kv_heads + a.groups - 1) / a.groups);
+}
+
+// 16 bytes a lane from `key` + `key_at` to LDS at `to` + 16 * lane, and from `value` + `value_at` to `gap` bytes
+// further, asynchronously: counted by vmcnt, with no register in flight.  (As a builtin, every LDS read would wait
+// for all of them.)  The idle cycles cover a scalar register that a vector instruction has just written, and m0.
+__device__ __forceinline__ void load_lds(const char* key, uint32_t key_at, const char* value, uint32_t value_at,
+                                         uint32_t to, uint32_t gap) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"
+      "global_load_lds_dwordx4 %4, %5" ::"s"(to), "v"(key_at), "s"(key), "s"(to + gap), "v"(value_at), "s"(value)
+      : "memory");
+}
+
+// Wait for all but the newest N of the wave's loads, then for the workgroup; LDS is ordered around it.
+template <int N>
+__device__ __forceinline__ void wait_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+// All but the newest `tiles` (at most MOST) of PER loads each.
+template <int PER, int MOST>
+__device__ __forceinline__ void wait_tiles(int tiles) {
+  if constexpr (MOST > 0)
+    if (tiles < MOST) return wait_tiles<PER, MOST - 1>(tiles);
+  wait_barrier<PER * MOST>();
+}
+// The same of LDS alone: loads stay in flight.
+__device__ __forceinline__ void lds_only_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <int E, int HD, int WQ, int WK, typename OutT>
+__global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_kernel(const TreeArgs a) {
+  using R = Ring<HD>;
+  constexpr int kNW = WQ * WK, kTile = R::kTile, kRows = 32 * WQ, kStages = R::kStages;
+  constexpr int kSub = kTile / (32 * WK);  // 32-position pieces of a tile that a wave takes
+  constexpr int kDT = HD / 32, kKS = HD / 16;
+  constexpr int kPos = kTile / kNW, kLoads = kPos / R::kGroup;  // a wave's positions of a tile, loads of K and of V
+  static_assert(kSub >= 1 && kLoads >= 1 && 2 * kLoads * (kStages - 1) < 64, "loads in flight that a wait can count");
+  constexpr int kKeys = 2;  // pieces of keys read at once
+  constexpr int kPer = kDT * 16 + 2;
+  static_assert((WK - 1) * WQ * kPer * 256 <= kStages * 2 * R::kBytes, "the joined sums fit the ring");
+  __shared__ __attribute__((aligned(1024))) char s_ring[2 * kStages * R::kBytes];  // stages of keys and of values
+  __shared__ __attribute__((aligned(8))) uint32_t s_mask[kRows][kWords];
+  __shared__ uint32_t s_bad[kWords];
+
+  const int id = (int)blockIdx.x;
+  const int group = id / (8 * a.row_blocks) * 8 + (id & 7);
+  const int rb = (id >> 3) % a.row_blocks;
+  if (group >= a.groups) return;
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qg = wave % WQ, kg = wave / WQ;
+  const int l32 = lane & 31, half = lane >> 5;
+  // Of the two waves on a SIMD one multiplies while the other takes its softmax: between the barriers of a step the
+  // first four of eight waves take products, then softmax, the others the softmax of the step before, then products.
+  constexpr bool kAlternate = kNW == 8;
+  const bool behind = kAlternate && wave >= 4;
+  if (id == 0)
+    for (int b = tid; b < a.batch; b += 64 * kNW)
+      if (a.seq_lens[b] > a.max_seq) atomicOr(a.errors, BARQ_KV_ERRBIT_ATTN_SHORT);
+
+  // ---- this group's range: [at, end) of the list; it begins in row b
+  int len_lane = lane < a.batch ? row_length(a, lane) : 0;  // of the 64 rows from len_row on
+  int len_row = 0;
+  asm volatile("" : "+v"(len_lane));  // waited for here, as below
+  int all = barq_commit::wave_sum(lane < a.batch ? pair_places<kTile>(a, len_lane) : 0);
+  for (int r0 = 64; r0 < a.batch; r0 += 64)
+    all += barq_commit::wave_sum(r0 + lane < a.batch ? pair_places<kTile>(a, row_length(a, r0 + lane)) : 0);
+  const int range = range_of(a, all);
+  int at = group * range;
+  const int end = min(at + range, all * a.kv_heads);
+  if (at >= end) return;
+  int b = 0, row_start = 0;  // row b's first place in the list
+  for (;;) {
+    const int here = len_row + lane < a.batch ? pair_places<kTile>(a, len_lane) * a.kv_heads : 0;
+    const int incl = barq_commit::wave_incl_scan(here);
+    const uint64_t past = __ballot(row_start + incl > at && here > 0);
+    if (past) {
+      const int k = __builtin_ctzll(past);
+      b = len_row + k;
+      row_start += __builtin_amdgcn_readlane(incl - here, k);
+      break;
+    }
+    row_start += __builtin_amdgcn_readlane(incl, 63);
+    len_row += 64;
+    len_lane = len_row + lane < a.batch ? row_length(a, len_row + lane) : 0;
+    asm volatile("" : "+v"(len_lane));
+  }
+
+  const int row = rb * kRows + qg * 32 + l32;  // query row: node * G + head of the group
+  const int node_row = (int)a.div_group.div((uint32_t)min(row, a.rows - 1));
+  const int group_head = min(row, a.rows - 1) - node_row * a.group;
+  const int node_lo = (int)a.div_group.div((uint32_t)(rb * kRows));
+  const bool wave_live = rb * kRows + qg * 32 < a.rows;
+  const int ntiles = (a.nodes + kTile - 1) / kTile;
+  // a lane's place in a load: position lane / kChunks of the group, and for the place of a piece in LDS the piece
+  // that belongs there
+  const int lp = lane / R::kChunks, slot_c = lane % R::kChunks;
+  const int node_c = tid % R::kChunks, node_p = tid / R::kChunks;
+  constexpr int kNodeStep = 64 * kNW / R::kChunks, kNodeLoads = kTile / kNodeStep;
+  // The lanes' places in a tile: of their key's piece of k-step 0 (step k: bits of k << 5 turned over) and of V's
+  // transposing read of dims 0 .. 31 (dims 32 d ..: bits of d << 6).  For that lane i of 16 gives the address of
+  // position i / 4 and dims 4 (i % 4), and gets dim i of the four positions.
+  const int vp = (lane & 15) >> 2;
+  const uint32_t key_lane = (uint32_t)key_at<HD>(kg * kSub * 32 + l32, half);
+  const uint32_t value_lane = (uint32_t)(R::kBytes + value_at<HD>(kg * kSub * 32 + 4 * half + vp,
+                                                                 ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) +
+                                         (lane & 1) * 8);
+  // and, from a wave's first position of a tile on, of what it loads: of a load's group of positions its own, and of
+  // that the piece that belongs in its place
+  const uint32_t key_from = (uint32_t)(lp * a.row_bytes) + (uint32_t)(slot_c ^ ((wave * kPos + lp) & (HD == 64 ? 7 : 15))) * 16;
+  const uint32_t value_from = (uint32_t)(lp * a.row_bytes) +
+                              (uint32_t)(slot_c ^ ((HD == 64 ? (lp >> 1) & 1 : (wave * kPos + lp) & 3) << 2)) * 16;
+  // turned over in these for the i-th group
+  constexpr auto key_turn = [](int i) { return (uint32_t)((i * R::kGroup) & (HD == 64 ? 7 : 15)) << 4; };
+  constexpr auto value_turn = [](int i) { return HD == 64 ? 0u : (uint32_t)((i * R::kGroup) & 3) << 6; };
+  const int block_step = kTile / (int)a.div_page.d, place_step = kTile % (int)a.div_page.d;  // of a tile
+  const bool whole = (int)a.div_page.d % kPos == 0;  // a wave's positions of a tile lie in one page
+
+  for (bool first = true; at < end;) {
+    if (b >= len_row + 64) {
+      len_row += 64;
+      len_lane = len_row + lane < a.batch ? row_length(a, len_row + lane) : 0;
+      asm volatile("" : "+v"(len_lane));
+    }
+    const int len = __builtin_amdgcn_readlane(len_lane, b - len_row);
+    const int tiles = pair_tiles<kTile>(a, len), places = tiles + kPairCost;
+    const int kvh = (at - row_start) / places;
+    if (kvh >= a.kv_heads) {  // the next row
+      row_start += places * a.kv_heads;
+      ++b;
+      continue;
+    }
+    const int pair_start = row_start + kvh * places + kPairCost;  // its first tile's place
+    const int t0 = max(at - pair_start, 0), t1 = min(tiles, end - pair_start);
+    at = pair_start + max(t1, 0);
+    if (t1 <= t0) break;  // the range ends before the pair's first tile
+    const int head = kvh * a.group + group_head;
+    const int count = t1 - t0, nodes_here = max(min(t1, ntiles) - t0, 0);  // tiles, and those of nodes, first
+    const int c0 = max(t0 - ntiles, 0);                                    // the first cached tile
+
+    // What a piece needs once is read again from the kernel's arguments: scalar registers are for the tiles.
+    const __attribute__((address_space(4))) TreeArgs* rare =
+        (const __attribute__((address_space(4))) TreeArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(rare));
+
+    u32x4 q[kKS];
+    {
+      const char* qp = rare->q + (int64_t)b * rare->q_sb + (int64_t)head * rare->q_sh + (int64_t)node_row * rare->q_st + half * 16;
+#pragma unroll
+      for (int k = 0; k < kKS; ++k) q[k] = *(const u32x4*)(qp + k * 32);
+    }
+
+    // ---- cached tiles: each wave loads kPos positions of a tile, a group of kGroup in one load
+    const int32_t* table = rare->block_table + (int64_t)b * rare->max_blocks;
+    const int last_blk = count > nodes_here ? (int)a.div_page.div((uint32_t)(len - 1)) : 0;
+    const auto entries = [&](int blk0) __attribute__((always_inline)) {  // a window of the block table, one entry a lane
+      const int e = blk0 + lane <= last_blk ? table[blk0 + lane] : 0;
+      if (e >= 0 && e < rare->num_pages) return e;
+      atomicOr(rare->errors, BARQ_KV_ERRBIT_BAD_INDEX);
+      return 0;
+    };
+    // The wave's block (place in it) of the next tile to load; the pages' offsets of 64 blocks from blk0 on and of
+    // the 64 after them, one a lane.
+    int blk0 = 0, blk = 0, place = 0;
+    int64_t window = 0, ahead = 0;
+    if (count > nodes_here) {
+      const int pos = c0 * kTile + wave * kPos;
+      blk = (int)a.div_page.div((uint32_t)pos);
+      place = pos - blk * (int)a.div_page.d;
+      blk0 = min(blk, last_blk);
+      window = (int64_t)entries(blk0) * a.page_bytes;
+      ahead = (int64_t)entries(blk0 + 64) * a.page_bytes;
+    }
+    // The query has come when the table has: waited for here, and not in the loop.
+#pragma unroll
+    for (int k = 0; k < kKS; ++k) asm volatile("" : "+v"(q[k]));
+    asm volatile("" : "+v"(window), "+v"(ahead));
+    const int64_t head_at = (int64_t)kvh * a.head_bytes;
+    // The piece's tile t of keys (V: of values) into its stage.  Nodes go through registers.
+    const auto load_nodes = [&](int t, bool v) __attribute__((always_inline)) {
+      char* const stage = s_ring + (2 * (t & (kStages - 1)) + (v ? 1 : 0)) * R::kBytes;
+      const char* const from = (v ? rare->nv : rare->nk) + (int64_t)b * rare->n_sb + (int64_t)kvh * rare->n_sh + node_c * 16;
+      u32x4 reg[kNodeLoads];
+#pragma unroll
+      for (int i = 0; i < kNodeLoads; ++i)
+        reg[i] = *(const u32x4*)(from + (int64_t)min((t0 + t) * kTile + node_p + i * kNodeStep, rare->nodes - 1) * rare->n_st);
+#pragma unroll
+      for (int i = 0; i < kNodeLoads; ++i) asm volatile("" : "+v"(reg[i]));  // waited for in any case
+#pragma unroll
+      for (int i = 0; i < kNodeLoads; ++i) {
+        const int p = node_p + i * kNodeStep, j = (t0 + t) * kTile + p;
+        if (v) {
+          bool keep = j < rare->nodes;
+          if (keep && nonfinite8<E>(reg[i])) {  // a V that is not finite is kept apart
+            atomicOr(&s_bad[j / 32], 1u << (j % 32));
+            keep = false;
+          }
+          *(u32x4*)(stage + value_at<HD>(p, node_c)) = keep ? reg[i] : u32x4{0, 0, 0, 0};
+        } else {
+          *(u32x4*)(stage + key_at<HD>(p, node_c)) = reg[i];
+        }
+      }
+    };
+    const char* const kbase = a.kpages + head_at;
+    const int64_t to_values = a.vpages - a.kpages;
+    typedef __attribute__((address_space(3))) char lds_char;
+    lds_char* const ring = (lds_char*)s_ring;
+    const uint32_t ring_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ring);
+    const auto page_of = [&](int i) __attribute__((always_inline)) {  // a block's page, i blocks after blk0
+      const int64_t w = i < 64 ? window : ahead;
+      const uint32_t lo32 = __builtin_amdgcn_readlane((int)(uint32_t)w, i & 63);
+      const uint32_t hi32 = __builtin_amdgcn_readlane((int)(w >> 32), i & 63);
+      return (int64_t)(((uint64_t)hi32 << 32) | lo32);
+    };
+    const auto load_cached = [&](int t) __attribute__((always_inline)) {  // tile t of the piece; in order
+      const uint32_t to = ring_at + (uint32_t)(t & (kStages - 1)) * (2 * R::kBytes) + (uint32_t)(wave * kPos * HD * 2);
+      const int base = (c0 + t - nodes_here) * kTile + wave * kPos;
+      if (blk >= blk0 + 64 && blk0 + 64 <= last_blk) {
+        blk0 += 64;
+        window = ahead;
+        ahead = (int64_t)entries(blk0 + 64) * a.page_bytes;
+      }
+      if (whole && base + kPos <= len) {
+        const char* const k0 = kbase + (page_of(blk - blk0) + (int64_t)place * a.row_bytes);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const char* const k = k0 + (int64_t)i * R::kGroup * a.row_bytes;
+          load_lds(k, key_from ^ key_turn(i), k + to_values, value_from ^ value_turn(i), to + i * 1024, R::kBytes);
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < kLoads; ++i) {
+          // past the row's end: its last group again, and in that its last position (never seen by a query)
+          const int pos = min(base + i * R::kGroup, (len - 1) / R::kGroup * R::kGroup);
+          const int bi = (int)a.div_page.div((uint32_t)pos);
+          const char* const k = kbase + (page_of(bi - blk0) + (int64_t)(pos - bi * (int)a.div_page.d) * a.row_bytes);
+          const uint32_t back = (uint32_t)(max(lp - (len - 1 - pos), 0) * a.row_bytes);
+          load_lds(k, (key_from ^ ((uint32_t)((i * R::kGroup) & (HD == 64 ? 7 : 15)) << 4)) - back, k + to_values,
+                   (value_from ^ (HD == 64 ? 0u : (uint32_t)((i * R::kGroup) & 3) << 6)) - back, to + i * 1024, R::kBytes);
+        }
+      }
+      blk += block_step;
+      place += place_step;
+      if (place >= (int)a.div_page.d) {
+        place -= (int)a.div_page.d;
+        ++blk;
+      }
+    };
+
+    f32x16 o[kDT], s[kSub];
+    u32x4 hi[kSub][2], lo[kSub][2];
+#pragma unroll
+    for (int d = 0; d < kDT; ++d) o[d] = f32x16{0};
+    float m = -INFINITY, l = 0.0f;
+
+    u32x4 key[2][kKeys];
+    const auto read_keys = [&](const lds_char* from, int n, u32x4 (&to)[kKeys]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i) {
+        const int u = (n * kKeys + i) / kKS, k = (n * kKeys + i) % kKS;
+        to[i] = *(const __attribute__((address_space(3))) u32x4*)((const lds_char*)(uintptr_t)((uint32_t)(uintptr_t)from ^ (uint32_t)(k << 5)) + u * 32 * HD * 2);
+      }
+    };
+    const auto key_stage = [&](int t) __attribute__((always_inline)) { return ring + (t & (kStages - 1)) * (2 * R::kBytes) + key_lane; };
+    constexpr int kKeyBatches = kSub * kKS / kKeys;
+
+    // ---- V of tile t times its probabilities
+    const auto weigh_values = [&](int t) __attribute__((always_inline)) {
+      typedef __attribute__((address_space(3))) s16x4 lds4;
+      const lds_char* const from = ring + (t & (kStages - 1)) * (2 * R::kBytes) + value_lane;
+      constexpr int kVals = 2, kBatches = 2 * kSub * (kDT / kVals);  // batches of 16 positions by 64 dims
+      u32x4 val[2][kVals];
+      const auto read_values = [&](int n, u32x4 (&to)[kVals]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kVals; ++i) {
+          const int d = n % (kDT / kVals) * kVals + i;
+          lds_char* const x = (lds_char*)(uintptr_t)((uint32_t)(uintptr_t)from ^ (uint32_t)(d << 6)) + n / (kDT / kVals) * 16 * HD * 2;
+          const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)x);
+          const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(x + 8 * HD * 2));
+          const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
+          to[i] = u32x4{w0[0], w0[1], w1[0], w1[1]};
+        }
+      };
+      read_values(0, val[0]);
+#pragma unroll
+      for (int n = 0; n < kBatches; ++n) {
+        if (n + 1 < kBatches) read_values(n + 1, val[(n + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);  // the next values are on their way while these are multiplied
+        const int p = n / (kDT / kVals), d0 = n % (kDT / kVals) * kVals;
+#pragma unroll
+        for (int i = 0; i < kVals; ++i) o[d0 + i] = mfma<E>(val[n & 1][i], lo[p / 2][p & 1], o[d0 + i]);
+#pragma unroll
+        for (int i = 0; i < kVals; ++i) o[d0 + i] = mfma<E>(val[n & 1][i], hi[p / 2][p & 1], o[d0 + i]);
+      }
+      if (t < nodes_here) {
+        asm volatile("" : "+s"(rare));  // nodes whose V is not finite, for the rows that see them alone
+#pragma unroll 1
+        for (int u = 0; u < kSub; ++u) {
+          const int jb = (t0 + t) * kTile + (kg * kSub + u) * 32;
+          uint32_t bad = jb < rare->nodes ? __builtin_amdgcn_readfirstlane(s_bad[jb / 32]) : 0u;
+          while (bad) {
+            const int j = __builtin_ctz(bad);
+            bad &= bad - 1;
+            float p = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kSub; ++w)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const uint32_t h = hi[w][i / 8][(i % 8) / 2], r = lo[w][i / 8][(i % 8) / 2];
+                const float x = i & 1 ? high_of<E>(h) + high_of<E>(r) : low_of<E>(h) + low_of<E>(r);
+                p = w == u && (j >> 3) * 4 + (j & 3) == i ? x : p;
+              }
+            const f32x2 both = halves(p);
+            p = j & 4 ? both[1] : both[0];
+            const char* vrow = rare->nv + (int64_t)b * rare->n_sb + (int64_t)kvh * rare->n_sh + (int64_t)(jb + j) * rare->n_st + half * 8;
+#pragma unroll
+            for (int d = 0; d < kDT; ++d)
+#pragma unroll
+              for (int w4 = 0; w4 < 4; ++w4) {
+                u32x2 w = *(const u32x2*)(vrow + d * 64 + w4 * 16);
+                asm volatile("" : "+v"(w));  // waited for here: never outstanding in the tiles' loop
+                if (p > 0.0f) {
+                  o[d][4 * w4] += p * low_of<E>(w[0]);
+                  o[d][4 * w4 + 1] += p * high_of<E>(w[0]);
+                  o[d][4 * w4 + 2] += p * low_of<E>(w[1]);
+                  o[d][4 * w4 + 3] += p * high_of<E>(w[1]);
+                }
+              }
+          }
+        }
+      }
+    };
+
+    // ---- the running maximum after tile t's scores (masked here); the sums follow it when it grows by 2^8
+    const auto raise = [&](int t, f32x16 (&x)[kSub]) __attribute__((always_inline)) {
+      const int valid = len - (c0 + t - nodes_here) * kTile;  // cached positions from the tile's first on
+      float top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) {
+        const int pb = (kg * kSub + u) * 32;
+        if (t < nodes_here || valid < pb + 32) {
+          uint32_t seen;
+          if (t < nodes_here) {
+            asm volatile("" : "+s"(rare));
+            const int jb = (t0 + t) * kTile + pb;
+            seen = jb < rare->nodes && row < rare->rows ? s_mask[node_row - node_lo][jb / 32] : 0u;
+          } else {
+            seen = valid <= pb ? 0u : (1u << (valid - pb)) - 1u;
+          }
+          seen >>= 4 * half;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[u][i] = seen >> (8 * (i / 4) + i % 4) & 1 ? x[u][i] : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, x[u][i]);
+      }
+      const f32x2 tops = halves(top);
+      top = fmaxf(tops[0], tops[1]) * a.scale_log2;
+      if (__any(top > m + 8.0f)) {
+        const float fresh = fmaxf(m, top);
+        const float by = fresh == -INFINITY ? 1.0f : exp2_(m - fresh);
+        m = fresh;
+        l *= by;
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) o[d] *= by;
+      }
+    };
+
+    // ---- scores of tile t
+    const auto score = [&](int t) __attribute__((always_inline)) {
+      const lds_char* const keys = key_stage(t);
+      read_keys(keys, 0, key[0]);
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) s[u] = f32x16{0};
+#pragma unroll
+      for (int n = 0; n < kKeyBatches; ++n) {
+        if (n + 1 < kKeyBatches) read_keys(keys, n + 1, key[(n + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i) {
+          const int u = (n * kKeys + i) / kKS, k = (n * kKeys + i) % kKS;
+          s[u] = mfma<E>(key[n & 1][i], q[k], s[u]);
+        }
+      }
+    };
+
+    // ---- probabilities of a tile against the running maximum, as pairs of 16-bit numbers
+    const auto weights = [&]() __attribute__((always_inline)) {
+      const float shift = m == -INFINITY ? 0.0f : -m;
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float p0 = exp2_(fmaf(s[u][i], a.scale_log2, shift)), p1 = exp2_(fmaf(s[u][i + 1], a.scale_log2, shift));
+          l += p0;
+          l += p1;
+          const uint32_t w = pack2<E>(p0, p1);
+          hi[u][i / 8][(i % 8) / 2] = w;
+          lo[u][i / 8][(i % 8) / 2] = pack2<E>(p0 - low_of<E>(w), p1 - high_of<E>(w));
+        }
+    };
+
+    // Keys of tile t are read in step t, values in step t + 1; its stage is loaded again in the step after.
+    if (!first) lds_only_barrier();  // the piece before is read from LDS
+    first = false;
+    constexpr int kAhead = kStages - 2;
+    const auto load_step = [&](int t) __attribute__((always_inline)) {
+      if (t + kAhead >= nodes_here && t + kAhead < count) load_cached(t + kAhead);
+    };
+    for (int t = nodes_here; t < min(count, kAhead); ++t) load_cached(t);
+    // tiles on their way when step t + 1 needs its own
+    const auto tiles_after = [&](int t) __attribute__((always_inline)) { return max(min(count - 1, t + kAhead) - (t + 1), 0); };
+    if (nodes_here > 0) {  // the tree's mask as bits
+      if (tid < kWords) s_bad[tid] = 0;
+      const int rows_here = (int)a.div_group.div((uint32_t)min(rb * kRows + kRows - 1, rare->rows - 1)) - node_lo + 1;
+      const int words = (rare->nodes + 63) / 64;  // of 64 nodes
+      constexpr int kMany = 4;                    // of them a wave has in flight
+      for (int i0 = wave * kMany; i0 < rows_here * words; i0 += kNW * kMany) {
+        uint8_t byte[kMany];
+#pragma unroll
+        for (int u = 0; u < kMany; ++u) {
+          const int i = min(i0 + u, rows_here * words - 1), n = node_lo + i / words, j = i % words * 64 + lane;
+          byte[u] = j <= n;
+          if (rare->mask)
+            byte[u] = rare->mask[(int64_t)b * rare->m_sb + (int64_t)n * rare->m_si + (int64_t)min(j, rare->nodes - 1) * rare->m_sj];
+        }
+#pragma unroll
+        for (int u = 0; u < kMany; ++u) {
+          const int i = min(i0 + u, rows_here * words - 1), j = i % words * 64 + lane;
+          const uint64_t bits = __ballot(byte[u] != 0 && j < rare->nodes);
+          if (lane == 0) *(uint64_t*)&s_mask[i / words][i % words * 2] = bits;
+        }
+      }
+      lds_only_barrier();  // s_bad is cleared
+    }
+    for (int t = 0; t < nodes_here; ++t) {  // at most kStages of them
+      load_nodes(t, false);
+      load_nodes(t, true);
+    }
+    wait_tiles<2 * kLoads, kAhead - 1>(min(count, kAhead) - 1);
+    asm volatile("" : "+s"(rare));
+    const auto softmax = [&](int t) __attribute__((always_inline)) {
+      raise(t, s);
+      weights();
+    };
+    const auto step_end = [&](int t) __attribute__((always_inline)) {
+      wait_tiles<2 * kLoads, kAhead - 1>(tiles_after(t));
+    };
+    const auto products = [&](int t) __attribute__((always_inline)) {
+      __builtin_amdgcn_s_setprio(1);
+      load_step(t);
+      weigh_values(t - 1);
+      score(t);
+      __builtin_amdgcn_s_setprio(0);
+    };
+    if (!wave_live) {  // no query rows: the loads alone
+      for (int t = 0; t < count; ++t) {
+        load_step(t);
+        step_end(t);
+      }
+    } else {
+      load_step(0);
+      score(0);
+      if (!behind) softmax(0);
+      step_end(0);
+      if (behind) {
+        for (int t = 1; t < count; ++t) {
+          softmax(t - 1);
+          products(t);
+          step_end(t);
+        }
+        softmax(count - 1);
+      } else {
+        for (int t = 1; t < count; ++t) {
+          products(t);
+          softmax(t);
+          step_end(t);
+        }
+      }
+      weigh_values(count - 1);
+    }
+    if constexpr (WK > 1) lds_only_barrier();  // every wave has read the ring
+    asm volatile("" : "+s"(rare));
+    const f32x2 ls = halves(l);
+    l = ls[0] + ls[1];
+
+    if constexpr (WK > 1) {  // join the groups of positions
+      float* s_join = (float*)s_ring;
+      if (kg > 0) {
+        float* to = s_join + ((kg - 1) * WQ + qg) * kPer * 64;
+#pragma unroll
+        for (int d = 0; d < kDT; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *(f32x4*)(to + (d * 4 + g) * 256 + lane * 4) =
+                f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+        to[kDT * 1024 + lane] = m;
+        to[kDT * 1024 + 64 + lane] = l;
+      }
+      lds_only_barrier();
+      if (kg == 0) {
+        float top = m, scale[WK];
+        scale[0] = m;
+#pragma unroll
+        for (int k = 1; k < WK; ++k) {
+          scale[k] = s_join[((k - 1) * WQ + qg) * kPer * 64 + kDT * 1024 + lane];
+          top = fmaxf(top, scale[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < WK; ++k) scale[k] = scale[k] == -INFINITY ? 0.0f : exp2_(scale[k] - top);
+        m = top;
+        l *= scale[0];
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) o[d] *= scale[0];
+#pragma unroll
+        for (int k = 1; k < WK; ++k) {
+          const float* from = s_join + ((k - 1) * WQ + qg) * kPer * 64;
+          l += scale[k] * from[kDT * 1024 + 64 + lane];
+#pragma unroll
+          for (int d = 0; d < kDT; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const f32x4 v = *(const f32x4*)(from + (d * 4 + g) * 256 + lane * 4);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[d][4 * g + e] += scale[k] * v[e];
+            }
+        }
+      }
+    }
+    if (kg > 0 || row >= rare->rows) continue;
+    if (t0 == 0 && t1 == tiles) {
+      const float by = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      char* op = rare->out + (int64_t)b * rare->o_sb + (int64_t)head * rare->o_sh + (int64_t)node_row * rare->o_st +
+                 half * 4 * (int)sizeof(OutT);
+#pragma unroll
+      for (int d = 0; d < kDT; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          store4<E, OutT>(op + (d * 32 + g * 8) * (int)sizeof(OutT),
+                          f32x4{o[d][4 * g] * by, o[d][4 * g + 1] * by, o[d][4 * g + 2] * by, o[d][4 * g + 3] * by});
+    } else {
+      const int64_t rec = (int64_t)(2 * group + (t0 == 0)) * rare->rows + row;
+      float* to = rare->part + rec * HD + half * 4;
+#pragma unroll
+      for (int d = 0; d < kDT; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *(f32x4*)(to + d * 32 + g * 8) = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+      if (half == 0) *(f32x2*)(rare->part_ml + rec * 2) = f32x2{m, l};
+    }
+  }
+}
+
+// Joins the records of a pair: HD / 4 threads a query row.
+template <int E, int HD, typename OutT>
+__global__ void __launch_bounds__(kThreads) tree_flat_join_kernel(const TreeArgs a) {
+  constexpr int kPer = kThreads / (HD / 4), kTile = Ring<HD>::kTile;
+  const int pair = (int)blockIdx.x;
+  const int b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
+  int before, all;
+  count_places<kTile>(a, b, (int)threadIdx.x & 63, &before, &all);
+  const int range = range_of(a, all);
+  const int tiles = pair_tiles<kTile>(a, row_length(a, b));
+  const int start = before * a.kv_heads + kvh * (tiles + kPairCost) + kPairCost;
+  const int g0 = start / range, g1 = (start + tiles - 1) / range;
+  if (g0 == g1) return;
+  const int row = (int)blockIdx.y * kPer + (int)threadIdx.x / (HD / 4);
+  const int d = ((int)threadIdx.x % (HD / 4)) * 4;
+  if (row >= a.rows) return;
+  const auto record = [&](int g) { return (int64_t)(2 * g + (g == g0)) * a.rows + row; };
+  float top = -INFINITY;
+  for (int g = g0; g <= g1; ++g) top = fmaxf(top, a.part_ml[record(g) * 2]);
+  f32x4 sum = {0, 0, 0, 0};
+  float l = 0.0f;
+#pragma unroll 4
+  for (int g = g0; g <= g1; ++g) {
+    const f32x2 ml = *(const f32x2*)(a.part_ml + record(g) * 2);
+    const f32x4 v = *(const f32x4*)(a.part + record(g) * HD + d);
+    const float by = ml[0] == -INFINITY ? 0.0f : exp2_(ml[0] - top);
+    sum += by * v;
+    l += by * ml[1];
+  }
+  const float by = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  const int node = (int)a.div_group.div((uint32_t)row);
+  store4<E, OutT>(a.out + (int64_t)b * a.o_sb + (int64_t)(kvh * a.group + row - node * a.group) * a.o_sh +
+                      (int64_t)node * a.o_st + d * (int)sizeof(OutT),
+                  sum * by);
+}
+
 struct Plan {
-  int wq, tile, row_blocks;
+  bool flat;
+  int wq, wk, tile, row_blocks, groups;
   int64_t splits, range, pairs, rows;
 };
 
 // How a call is cut: query rows by the fewest blocks, then ranges of tiles so that the launch fills the GPU.
-bool plan_of(const barq_kv_pool* p, int64_t batch, int64_t q_heads, int64_t nodes, int64_t max_seq, int64_t mean_seq,
-             Plan* out) {
+bool plan_of(const barq_kv_pool* p, bool cold, int64_t batch, int64_t q_heads, int64_t nodes, int64_t max_seq,
+             int64_t mean_seq, Plan* out) {
   if (!p || p->elem_bytes != 2 || (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)) return false;
   if (p->kv_heads < 1 || batch < 1 || batch > p->max_batch || q_heads < 1 || q_heads % p->kv_heads || nodes < 1 ||
       nodes > BARQ_TREE_MAX_NODES || max_seq < 0 || mean_seq < 0)
@@ -578,6 +1214,21 @@ bool plan_of(const barq_kv_pool* p, int64_t batch, int64_t q_heads, int64_t node
   const int64_t longest = max_seq == 0 ? cap : std::min(max_seq, cap);
   const int64_t rows = q_heads / p->kv_heads * nodes;
   if (rows > (int64_t(1) << 17)) return false;
+  const int64_t hd = p->head_dim, pairs_ = batch * p->kv_heads;
+  // Tiles by asynchronous loads: a load's group of positions lies in one page (their offsets in 32 bits).
+  out->flat = !cold && p->page_size % (512 / hd) == 0 && p->kv_heads * hd * 2 < (int64_t(1) << 27) &&
+              nodes <= (hd == 256 ? 128 : 256);  // its stages hold a tree at once
+  if (out->flat) {
+    const int wq = rows > 128 && hd != 256 ? 8 : rows > 64 ? 4 : rows > 32 || hd == 256 ? 2 : 1;
+    const int64_t blocks = (rows + 32 * wq - 1) / (32 * wq), kt = hd == 256 ? 32 : 64;
+    out->wq = wq;
+    out->wk = hd == 256 || wq == 8 ? 1 : 2;
+    out->row_blocks = (int)blocks;
+    out->groups = (int)std::max<int64_t>(1, 256 / blocks);  // one workgroup a compute unit
+    out->pairs = pairs_;
+    out->rows = rows;
+    return pairs_ * ((longest + kt - 1) / kt + (nodes + kt - 1) / kt) < (int64_t(1) << 30);
+  }
   const int wq = rows > 64 ? 4 : rows > 32 || p->head_dim == 256 ? 2 : 1;
   const int tile = wq == 1 ? 128 : 64;
   const int64_t pairs = batch * p->kv_heads, blocks = (rows + 32 * wq - 1) / (32 * wq);
@@ -598,6 +1249,7 @@ bool plan_of(const barq_kv_pool* p, int64_t batch, int64_t q_heads, int64_t node
 }
 
 int64_t workspace_of(const Plan& p, int64_t hd) {
+  if (p.flat) return 2 * (int64_t)p.groups * p.rows * (hd + 2) * 4;
   return p.splits == 1 ? 0 : p.pairs * p.splits * p.rows * (hd + 2) * 4;
 }
 
@@ -621,8 +1273,30 @@ Kernel join_of(int64_t hd) {
                      : (Kernel)&tree_join_kernel<E, 64, OutT>;
 }
 
-int launch(Kernel kernel, dim3 grid, void** args, void* stream) {
-  if (hipLaunchKernel(kernel, grid, dim3(kThreads), args, 0, (hipStream_t)stream) == hipSuccess) return BARQ_KV_OK;
+template <int E, int HD, typename OutT>
+Kernel flat_by_shape(const Plan& p) {
+  if constexpr (HD == 256) {
+    return p.wq == 4 ? (Kernel)&tree_flat_kernel<E, 256, 4, 1, OutT> : (Kernel)&tree_flat_kernel<E, 256, 2, 1, OutT>;
+  } else {
+    return p.wq == 8   ? (Kernel)&tree_flat_kernel<E, HD, 8, 1, OutT>
+           : p.wq == 4 ? (Kernel)&tree_flat_kernel<E, HD, 4, 2, OutT>
+           : p.wq == 2 ? (Kernel)&tree_flat_kernel<E, HD, 2, 2, OutT>
+                       : (Kernel)&tree_flat_kernel<E, HD, 1, 2, OutT>;
+  }
+}
+template <int E, typename OutT>
+Kernel flat_by_head(int64_t hd, const Plan& p) {
+  return hd == 256 ? flat_by_shape<E, 256, OutT>(p) : hd == 128 ? flat_by_shape<E, 128, OutT>(p) : flat_by_shape<E, 64, OutT>(p);
+}
+template <int E, typename OutT>
+Kernel flat_join_of(int64_t hd) {
+  return hd == 256   ? (Kernel)&tree_flat_join_kernel<E, 256, OutT>
+         : hd == 128 ? (Kernel)&tree_flat_join_kernel<E, 128, OutT>
+                     : (Kernel)&tree_flat_join_kernel<E, 64, OutT>;
+}
+
+int launch(Kernel kernel, dim3 grid, void** args, void* stream, int threads = kThreads) {
+  if (hipLaunchKernel(kernel, grid, dim3((uint32_t)threads), args, 0, (hipStream_t)stream) == hipSuccess) return BARQ_KV_OK;
   (void)hipGetLastError();
   return BARQ_KV_ERR_LAUNCH;
 }
@@ -631,10 +1305,10 @@ int launch(Kernel kernel, dim3 grid, void** args, void* stream) {
 
 extern "C" {
 
-int64_t barq_tree_attention_workspace_bytes(const barq_kv_pool* pool, int64_t batch, int64_t q_heads, int64_t nodes,
+int64_t barq_tree_attention_workspace_bytes(const barq_kv_pool* pool, int64_t cold, int64_t batch, int64_t q_heads, int64_t nodes,
                                             int64_t max_seq, int64_t mean_seq) {
   Plan p;
-  return plan_of(pool, batch, q_heads, nodes, max_seq, mean_seq, &p) ? workspace_of(p, pool->head_dim) : -1;
+  return plan_of(pool, cold != 0, batch, q_heads, nodes, max_seq, mean_seq, &p) ? workspace_of(p, pool->head_dim) : -1;
 }
 
 int barq_tree_attention(const barq_kv_pool* pool, const barq_kv_cold* cold, const void* query, int64_t batch,
@@ -649,7 +1323,7 @@ int barq_tree_attention(const barq_kv_pool* pool, const barq_kv_cold* cold, cons
       !query || !node_key || !node_value || !out || (flags & ~(int64_t)(BARQ_KV_ATTN_FP16 | BARQ_KV_ATTN_OUT_F32)) ||
       pool->num_pages < 1 || pool->num_pages > kI32Max || pool->page_size < 1 || pool->max_blocks < 1 ||
       pool->max_blocks * pool->page_size > kI32Max || pool->kv_heads * pool->head_dim * 2 > kI32Max ||
-      !plan_of(pool, batch, q_heads, nodes, max_seq, mean_seq, &plan))
+      !plan_of(pool, cold != nullptr, batch, q_heads, nodes, max_seq, mean_seq, &plan))
     return BARQ_KV_ERR_INVALID;
   const bool f16 = flags & BARQ_KV_ATTN_FP16, f32 = flags & BARQ_KV_ATTN_OUT_F32;
   const int64_t os = f32 ? 4 : 2, hd = pool->head_dim;
@@ -689,7 +1363,9 @@ int barq_tree_attention(const barq_kv_pool* pool, const barq_kv_cold* cold, cons
   a.m_sb = mask_stride_b, a.m_si = mask_stride_i, a.m_sj = mask_stride_j;
   a.o_sb = out_stride_b * os, a.o_sh = out_stride_h * os, a.o_st = out_stride_t * os;
   a.part = (float*)workspace;
-  a.part_ml = a.part + plan.pairs * plan.splits * plan.rows * hd;
+  a.part_ml = a.part + (plan.flat ? 2 * plan.groups : plan.pairs * plan.splits) * plan.rows * hd;
+  a.batch = (int32_t)batch;
+  a.groups = plan.groups;
   a.group = (int32_t)(q_heads / pool->kv_heads);
   a.div_page = FastDiv::make((uint32_t)pool->page_size);
   a.div_group = FastDiv::make((uint32_t)a.group);
@@ -712,6 +1388,18 @@ int barq_tree_attention(const barq_kv_pool* pool, const barq_kv_cold* cold, cons
     a.kscales = (const uint8_t*)cold->key_scales;
     a.vscales = (const uint8_t*)cold->value_scales;
     a.num_cold = (int32_t)cold->num_cold;
+  }
+  if (plan.flat) {
+    const Kernel flat = f16 ? (f32 ? flat_by_head<kF16, float>(hd, plan) : flat_by_head<kF16, uint16_t>(hd, plan))
+                            : (f32 ? flat_by_head<kBF16, float>(hd, plan) : flat_by_head<kBF16, uint16_t>(hd, plan));
+    const Kernel join = f16 ? (f32 ? flat_join_of<kF16, float>(hd) : flat_join_of<kF16, uint16_t>(hd))
+                            : (f32 ? flat_join_of<kBF16, float>(hd) : flat_join_of<kBF16, uint16_t>(hd));
+    void* args[] = {&a};
+    const int64_t per = kThreads / (hd / 4);
+    const int rc = launch(flat, dim3((uint32_t)((plan.groups + 7) / 8 * 8 * plan.row_blocks)), args, stream,
+                          64 * plan.wq * plan.wk);
+    if (rc != BARQ_KV_OK) return rc;
+    return launch(join, dim3((uint32_t)plan.pairs, (uint32_t)((plan.rows + per - 1) / per)), args, stream);
   }
   const Kernel kernel = f16 ? (f32 ? by_head<kF16, float>(hd, cold, plan.wq) : by_head<kF16, uint16_t>(hd, cold, plan.wq))
                             : (f32 ? by_head<kBF16, float>(hd, cold, plan.wq) : by_head<kBF16, uint16_t>(hd, cold, plan.wq));

@@ -88,9 +88,9 @@ int barq_tree_attention(const barq_kv_pool* pool, const barq_kv_cold* cold, cons
                         int64_t out_stride_t, float scale, int64_t max_seq, int64_t mean_seq, int64_t flags,
                         void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Bytes of workspace barq_tree_attention needs (0: none), or -1 for arguments it rejects. */
-int64_t barq_tree_attention_workspace_bytes(const barq_kv_pool* pool, int64_t batch, int64_t q_heads, int64_t nodes,
-                                            int64_t max_seq, int64_t mean_seq);
+/* Bytes of workspace barq_tree_attention needs (0: none; cold: whether it is given one), or -1 for arguments it rejects. */
+int64_t barq_tree_attention_workspace_bytes(const barq_kv_pool* pool, int64_t cold, int64_t batch, int64_t q_heads,
+                                            int64_t nodes, int64_t max_seq, int64_t mean_seq);
 
 #ifdef __cplusplus
 }

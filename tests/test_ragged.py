@@ -110,8 +110,8 @@ def test_invalid_arguments_are_refused_before_any_launch(built):
     assert tree(good, out=ctypes.c_void_p(0x7F0000000004)) == 1 and tree(good, flags=4) == 1
     assert tree(good, max_seq=-1) == 1
     long = fake_pool(max_blocks=512)
-    assert built.barq_tree_attention_workspace_bytes(ctypes.byref(long), 1, 32, 4, 0, 0) > 0
-    assert built.barq_tree_attention_workspace_bytes(ctypes.byref(long), 1, 33, 4, 0, 0) == -1
+    assert built.barq_tree_attention_workspace_bytes(ctypes.byref(long), 0, 1, 32, 4, 0, 0) > 0
+    assert built.barq_tree_attention_workspace_bytes(ctypes.byref(long), 0, 1, 33, 4, 0, 0) == -1
     assert tree(long, batch=1, ws_bytes=0) == 1 and tree(long, batch=1, ws=None) == 1
     cold = _capi.BarqKVCold(*([0x7F0000000000] * 6), 16, 128, 1)  # fp16 codes of a bf16 call
     assert tree(good, cold=ctypes.byref(cold)) == 1
