@@ -9,6 +9,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
+#include <cstring>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -844,72 +845,116 @@ void pool_decode_attention_cold(std::vector<at::Tensor> pool, std::vector<at::Te
   decode_attention_into(pool, &c, query, out, scale, max_seq, split_tokens, workspace);
 }
 
+// A shadow's entries, by the buffer protocol itself: a model has two shadows a layer, and a described buffer costs
+// several times the copy of its rows.
+int64_t* shadow_of(PyObject* b, int64_t rows) {
+  Py_buffer v;
+  if (PyObject_GetBuffer(b, &v, PyBUF_CONTIG) != 0) throw py::error_already_set();
+  int64_t* const at = static_cast<int64_t*>(v.buf);
+  const bool ok = v.itemsize == 8 && v.len >= rows * 8;
+  PyBuffer_Release(&v);  // the caller's list keeps the array
+  TORCH_CHECK(ok, "a pool's host shadow is contiguous int64 arrays of at least batch entries");
+  return at;
+}
+
+// The whole numbers 0 .. limit of a list or tuple; false where anything else is in it.
+bool small_ints(const py::object& seq, int64_t limit, std::vector<int32_t>* to) {
+  if (!PyList_CheckExact(seq.ptr()) && !PyTuple_CheckExact(seq.ptr())) return false;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq.ptr());
+  PyObject** const item = PySequence_Fast_ITEMS(seq.ptr());
+  to->resize(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (!PyLong_CheckExact(item[i])) return false;
+    int past = 0;
+    const int64_t v = PyLong_AsLongLongAndOverflow(item[i], &past);
+    if (past || v < 0 || v > limit) return false;
+    (*to)[i] = (int32_t)v;
+  }
+  return true;
+}
+
 // lengths[i] new tokens into row rows[i] (or i) of a group's pools, checked against the pools' host shadows
 // (lens, hws: updated in place; free_counts: at least so many pages are free): (slots, positions, requests,
 // offsets, pages taken of each pool), or None, nothing done, when the checked Python path must look at the call.
-py::object pool_map_slots_(const at::Tensor& group, const at::Tensor& pages, const c10::optional<std::vector<int64_t>>& rows,
-                           const std::vector<int64_t>& lengths, const std::vector<py::buffer>& lens,
-                           const std::vector<py::buffer>& hws, const std::vector<int64_t>& free_counts, int64_t limit,
-                           bool layers) {
+py::object pool_map_slots_(const at::Tensor& group, const at::Tensor& pages, const py::object& rows,
+                           const py::object& lengths, const py::list& lens, const py::list& hws,
+                           const std::vector<int64_t>& free_counts, int64_t limit, bool layers) {
   int64_t num = 0;
   const barq_kv_pool* pools = group_pools(group, &num);
   const barq_kv_pool& g = pools[0];
   TORCH_CHECK(pages.is_cuda() && pages.data_ptr() == g.key_pages, "pages do not belong to the group");
-  const int64_t n = (int64_t)lengths.size();
   TORCH_CHECK((int64_t)lens.size() == num && (int64_t)hws.size() == num && (int64_t)free_counts.size() == num,
               "pool_map_slots_: one shadow per pool");
-  if ((rows && (int64_t)rows->size() != n) || n > g.max_batch) return py::none();
   limit = std::min(limit, g.max_blocks * g.page_size);
-  std::vector<int32_t> r32(n), n32(n);
-  int64_t total = 0;
-  for (int64_t i = 0; i < n; ++i) {
-    const int64_t r = rows ? (*rows)[i] : i;
-    if (r < 0 || r >= g.max_batch || lengths[i] < 0 || lengths[i] > limit) return py::none();
-    r32[i] = (int32_t)r;
-    n32[i] = (int32_t)lengths[i];
-    total += lengths[i];
-  }
-  if (total >= (int64_t(1) << 30)) return py::none();
-  if (rows) {
+  std::vector<int32_t> r32, n32;
+  if (g.max_blocks * g.page_size >= (int64_t(1) << 31) || !small_ints(lengths, limit, &n32)) return py::none();
+  const int64_t n = (int64_t)n32.size();
+  if (n > g.max_batch) return py::none();
+  if (rows.is_none()) {
+    r32.resize(n);
+    for (int64_t i = 0; i < n; ++i) r32[i] = (int32_t)i;
+  } else {
+    if (!small_ints(rows, g.max_batch - 1, &r32) || (int64_t)r32.size() != n) return py::none();
     std::vector<bool> seen(g.max_batch);
     for (const int32_t r : r32) {
       if (seen[r]) return py::none();
       seen[r] = true;
     }
   }
+  int64_t total = 0;
+  for (const int32_t k : n32) total += k;
+  if (total >= (int64_t(1) << 30)) return py::none();
   std::vector<int64_t*> L(num), W(num);
   std::vector<int64_t> need(num, 0);
+  std::vector<char> like_first(num, 0);  // the layer's shadow equals the first's, as those of a model do
+  const size_t bytes = (size_t)g.max_batch * 8;
   for (int64_t l = 0; l < num; ++l) {
     const barq_kv_pool& p = pools[l];
     if (p.max_batch != g.max_batch || p.max_blocks != g.max_blocks || p.page_size != g.page_size) return py::none();
-    L[l] = shadow(lens[l], g.max_batch);
-    W[l] = shadow(hws[l], g.max_batch);
+    L[l] = shadow_of(PyList_GET_ITEM(lens.ptr(), l), g.max_batch);
+    W[l] = shadow_of(PyList_GET_ITEM(hws.ptr(), l), g.max_batch);
     for (int64_t m = 0; m < l; ++m)
       if (L[m] == L[l]) return py::none();
-    for (int64_t i = 0; i < n; ++i) {
-      const int64_t r = r32[i], end = L[l][r] + n32[i];
-      if (L[l][r] != L[0][r] || (n32[i] > 0 && end > limit)) return py::none();
-      if (n32[i] > 0)
-        need[l] += std::max<int64_t>((end + p.page_size - 1) / p.page_size - (W[l][r] + p.page_size - 1) / p.page_size, 0);
+    like_first[l] = l > 0 && !std::memcmp(L[l], L[0], bytes) && !std::memcmp(W[l], W[0], bytes);
+    if (like_first[l]) {
+      need[l] = need[0];
+    } else {
+      const uint32_t P = (uint32_t)p.page_size;
+      for (int64_t i = 0; i < n; ++i) {
+        const int64_t r = r32[i], end = L[l][r] + n32[i];
+        if (L[l][r] != L[0][r] || (n32[i] > 0 && end > limit)) return py::none();
+        if (n32[i] > 0) {
+          const uint32_t last = (uint32_t)end / P + ((uint32_t)end % P != 0);
+          const uint32_t held = (uint32_t)W[l][r] / P + ((uint32_t)W[l][r] % P != 0);
+          need[l] += last > held ? last - held : 0;
+        }
+      }
     }
     if (need[l] > free_counts[l]) return py::none();
   }
   c10::DeviceGuard guard(pages.device());
   const auto wide = pages.options().dtype(at::kLong), narrow = pages.options().dtype(at::kInt);
   at::Tensor slots = layers ? at::empty({num, total}, wide) : at::empty({total}, wide);
-  at::Tensor both = at::empty({2, total}, narrow), offsets = at::empty({n + 1}, narrow);
+  at::Tensor positions = at::empty({total}, narrow), requests = at::empty({total}, narrow);
+  at::Tensor offsets = at::empty({n + 1}, narrow);
   if (n == 0) offsets.zero_();
-  check_status(barq_map_slots(pools, num, rows ? r32.data() : nullptr, n32.data(), n, slots.data_ptr<int64_t>(), total,
-                              both.data_ptr<int32_t>(), both.data_ptr<int32_t>() + total, offsets.data_ptr<int32_t>(),
-                              current_stream(pages)),
+  check_status(barq_map_slots(pools, num, rows.is_none() ? nullptr : r32.data(), n32.data(), n,
+                              slots.data_ptr<int64_t>(), total, positions.data_ptr<int32_t>(),
+                              requests.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), current_stream(pages)),
                "pool_map_slots_");
-  for (int64_t l = 0; l < num; ++l)
+  for (int64_t l = 0; l < num; ++l) {
+    if (like_first[l]) {  // the first's rows have advanced
+      std::memcpy(L[l], L[0], bytes);
+      std::memcpy(W[l], W[0], bytes);
+      continue;
+    }
     for (int64_t i = 0; i < n; ++i) {
       int64_t& len = L[l][r32[i]];
       len += n32[i];
       W[l][r32[i]] = std::max(W[l][r32[i]], len);
     }
-  return py::make_tuple(slots, both[0], both[1], offsets, need);
+  }
+  return py::make_tuple(slots, positions, requests, offsets, need);
 }
 
 // False, nothing done, when the checked Python path must look at the call.

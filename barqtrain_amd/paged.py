@@ -24,6 +24,7 @@ algorithm (same page-allocation order) written with torch CPU operators.
 from __future__ import annotations
 
 import math
+import operator
 from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
@@ -1283,7 +1284,8 @@ def _pool_group(pools: list[PagePool]):
             _GROUPS.clear()
         # the entry holds the pools, so the ids in its key stay theirs
         entry = {"pools": list(pools), "group": _gpu_backend().pool_group([p.tensors for p in pools]),
-                 "ws": None}
+                 "plain": (all(p.device == pools[0].device for p in pools)
+                           and not any(getattr(p, "quantized", False) for p in pools)), "ws": None}
         _GROUPS[key] = entry
     return entry
 
@@ -1342,10 +1344,10 @@ def _packed_copy(t: torch.Tensor) -> torch.Tensor:
 def _host_ints(values, what: str) -> list[int]:
     if isinstance(values, torch.Tensor) and values.device.type != "cpu":
         raise ValueError(f"map_slots: {what} are host numbers (a device tensor would be read with a synchronisation)")
-    values = values.tolist() if hasattr(values, "tolist") else [int(v) for v in values]
-    if any(not isinstance(v, int) for v in values):
-        raise ValueError(f"map_slots: {what} must be a flat sequence of whole numbers")
-    return values
+    try:
+        return list(map(operator.index, values.tolist() if hasattr(values, "tolist") else values))
+    except TypeError:
+        raise ValueError(f"map_slots: {what} must be a flat sequence of whole numbers") from None
 
 
 def map_slots_layers(pools: Sequence[PagePool], lengths: Sequence[int], rows: Optional[Sequence[int]] = None,
@@ -1359,23 +1361,29 @@ def map_slots_layers(pools: Sequence[PagePool], lengths: Sequence[int], rows: Op
 def _map_slots(pools: list, lengths, rows, max_length: Optional[int], layers: bool, retried: bool = False) -> SlotMap:
     if not pools:
         raise ValueError("map_slots: no pools")
-    lengths = _host_ints(lengths, "lengths")
-    rows = None if rows is None else _host_ints(rows, "rows")
     g = pools[0]
-    if any(getattr(p, "quantized", False) for p in pools):
-        _check_map(pools, lengths, rows, max_length, False)
-        for p in pools:
-            if getattr(p, "quantized", False):
-                p._settle()
-    if g.on_gpu and all(p.device == g.device for p in pools):
-        handle = g._packed() if len(pools) == 1 else (0, _pool_group(pools)["group"], None, _gpu_backend())
+    if not isinstance(lengths, (list, tuple)):  # lists and tuples are read by the binding, or below
+        lengths = _host_ints(lengths, "lengths")
+    if rows is not None and not isinstance(rows, (list, tuple)):
+        rows = _host_ints(rows, "rows")
+    entry = _GROUPS.get(tuple((id(p), p.generation) for p in pools)) if len(pools) > 1 else None
+    if entry is None or not entry["plain"]:
+        lengths, rows = _host_ints(lengths, "lengths"), None if rows is None else _host_ints(rows, "rows")
+        if any(getattr(p, "quantized", False) for p in pools):
+            _check_map(pools, lengths, rows, max_length, False)
+            for p in pools:
+                if getattr(p, "quantized", False):
+                    p._settle()
+    if entry is not None or (g.on_gpu and all(p.device == g.device for p in pools)):
+        group = g._packed()[1] if len(pools) == 1 else (entry or _pool_group(pools))["group"]
         limit = g.capacity if max_length is None else int(max_length)
-        got = handle[3].pool_map_slots_(handle[1], g.key_pages, rows, lengths, [p.lens for p in pools],
-                                        [p.hw for p in pools], [p.free_count for p in pools], limit, layers)
+        got = _gpu_backend().pool_map_slots_(group, g.key_pages, rows, lengths, [p.lens for p in pools],
+                                             [p.hw for p in pools], [p.free_count for p in pools], limit, layers)
         if got is not None:
             for p, need in zip(pools, got[4]):
                 p.free_count -= need
             return SlotMap(*got[:4])
+    lengths, rows = _host_ints(lengths, "lengths"), None if rows is None else _host_ints(rows, "rows")
     need = _check_map(pools, lengths, rows, max_length)
     if g.on_gpu:  # only a lower bound of the free pages stood in the way, and is exact now
         if retried:
