@@ -166,11 +166,9 @@ __device__ __forceinline__ int value_at(int p, int c) {
   return p * (HD * 2) + ((c ^ ((HD == 64 ? (p >> 1) & 1 : p & 3) << 2)) << 4);
 }
 
-// A page's entry as an index of pages (or, cold, -2 - cold page), 0 and flagged where it names none.
-template <bool COLD>
+// A page's entry as an index of pages, 0 and flagged where it names none.
 __device__ __forceinline__ int checked_entry(const TreeArgs& a, int e) {
   if (e >= 0 && e < a.num_pages) return e;
-  if (COLD && e <= -2 && -2 - e < a.num_cold) return e;
   atomicOr(a.errors, BARQ_KV_ERRBIT_BAD_INDEX);
   return 0;
 }
@@ -181,7 +179,7 @@ __device__ __forceinline__ void store4(char* p, const f32x4 v) {
   else *(u32x2*)p = u32x2{pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3])};
 }
 
-template <int E, int HD, int WQ, bool COLD, typename OutT>
+template <int E, int HD, int WQ, typename OutT>
 __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2) tree_kernel(const TreeArgs a) {
   using S = Shape<HD, WQ>;
   constexpr int kDT = HD / 32;     // 32-dim tiles of the output
@@ -253,8 +251,6 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2) tree_kernel(const
   const int32_t* table = a.block_table + (int64_t)b * a.max_blocks;
   int entry[S::kLoads];
   u32x4 kreg[S::kLoads], vreg[S::kLoads];
-  uint32_t cold_mask = 0, vshift = 0;  // of the tile in the registers
-  (void)vshift;
   auto load_entries = [&](int tile) {
     if (tile >= ctiles) return;
 #pragma unroll
@@ -262,42 +258,18 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2) tree_kernel(const
       entry[i] = table[a.div_page.div((uint32_t)min(tile * S::kTile + p0 + i * S::kStep, len - 1))];
   };
   auto load_tile = [&](int tile) {
-    cold_mask = 0;
     if (tile < ctiles) {
       int64_t at[S::kLoads];
 #pragma unroll
       for (int i = 0; i < S::kLoads; ++i) {
         const int pos = min(tile * S::kTile + p0 + i * S::kStep, len - 1);
-        const int e = checked_entry<COLD>(a, entry[i]);
         const int off = pos - (int)a.div_page.div((uint32_t)pos) * (int)a.div_page.d;
-        if constexpr (COLD) {
-          const bool cold = e < 0;
-          const int64_t cp = -2 - (int64_t)e;
-          cold_mask |= (uint32_t)cold << i;
-          // 8 bytes of codes and 8 of scales, or 16 of elements
-          const int64_t el = (cp * a.page_size + off) * (a.row_bytes / 2) + (int64_t)kvh * HD + c * 8;
-          const int64_t ks = (cp * a.kv_heads + kvh) * HD + c * 8;
-          const int64_t vs = ((cp * a.page_size + off) * a.kv_heads + kvh);
-          const int64_t hot = (int64_t)e * a.page_bytes + (int64_t)off * a.row_bytes + (int64_t)kvh * a.head_bytes + c * 16;
-          const char* k0 = cold ? (const char*)a.kcodes + el : a.kpages + hot;
-          const char* k1 = cold ? (const char*)a.kscales + ks : a.kpages + hot + 8;
-          const char* v0 = cold ? (const char*)a.vcodes + el : a.vpages + hot;
-          const char* v1 = cold ? (const char*)a.vscales + (vs & ~(int64_t)7) : a.vpages + hot + 8;
-          const u32x2 ka = *(const u32x2*)k0, kb = *(const u32x2*)k1;
-          const u32x2 va = *(const u32x2*)v0, vb = *(const u32x2*)v1;
-          kreg[i] = u32x4{ka[0], ka[1], kb[0], kb[1]};
-          vreg[i] = u32x4{va[0], va[1], vb[0], vb[1]};
-          at[i] = 0;
-        } else {
-          at[i] = (int64_t)e * a.page_bytes + (int64_t)off * a.row_bytes + (int64_t)kvh * a.head_bytes + c * 16;
-        }
+        at[i] = (int64_t)checked_entry(a, entry[i]) * a.page_bytes + (int64_t)off * a.row_bytes + (int64_t)kvh * a.head_bytes + c * 16;
       }
-      if constexpr (!COLD) {
 #pragma unroll
-        for (int i = 0; i < S::kLoads; ++i) {
-          kreg[i] = *(const u32x4*)(a.kpages + at[i]);
-          vreg[i] = *(const u32x4*)(a.vpages + at[i]);
-        }
+      for (int i = 0; i < S::kLoads; ++i) {
+        kreg[i] = *(const u32x4*)(a.kpages + at[i]);
+        vreg[i] = *(const u32x4*)(a.vpages + at[i]);
       }
     } else {
       const int64_t base = (int64_t)b * a.n_sb + (int64_t)kvh * a.n_sh + c * 16;
@@ -314,20 +286,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2) tree_kernel(const
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
       const int p = p0 + i * S::kStep;
-      u32x4 k = kreg[i], v = vreg[i];
-      if constexpr (COLD) {
-        if (cold_mask >> i & 1) {
-          uint32_t w[4];
-          barq_fp8::dequant8<E>(k[0], k[1], k[2], k[3], w);
-          k = u32x4{w[0], w[1], w[2], w[3]};
-          const int pos = min(tile * S::kTile + p, len - 1);
-          const int off = pos - (int)a.div_page.div((uint32_t)pos) * (int)a.div_page.d;
-          const int byte = (off * a.kv_heads + kvh) & 7;  // a page's scales begin at a multiple of 8
-          const uint32_t s = ((byte & 4 ? v[3] : v[2]) >> (byte & 3) * 8 & 0xFFu) * 0x01010101u;
-          barq_fp8::dequant8<E>(v[0], v[1], s, s, w);
-          v = u32x4{w[0], w[1], w[2], w[3]};
-        }
-      }
+      const u32x4 k = kreg[i], v = vreg[i];
       bool keep = p < limit;
       if (tile >= ctiles && keep && nonfinite8<E>(v)) {
         const int j = (tile - ctiles) * S::kTile + p;
@@ -570,9 +529,9 @@ __global__ void __launch_bounds__(kThreads) tree_join_kernel(const TreeArgs a, i
 // one list; group g of row_blocks workgroups takes the g-th equal range of it, whatever the rows' lengths.
 // A range's piece of a pair that is not the whole pair leaves a record (slot 2g for a piece that begins inside its
 // pair, else 2g + 1: a range has at most one of each), joined by a second launch in the order of the groups.
-template <int HD>
+template <int HD, int TILE>
 struct Ring {
-  static constexpr int kTile = HD == 256 ? 32 : 64;  // positions of a tile
+  static constexpr int kTile = TILE;                 // positions of a tile
   static constexpr int kBytes = kTile * HD * 2;      // of its keys, or values
   static constexpr int kStages = 65536 / kBytes;     // tiles in LDS: 128 KB of them
   static constexpr int kChunks = HD / 8;
@@ -587,7 +546,7 @@ __device__ __forceinline__ int pair_tiles(const TreeArgs& a, int len) {
 }
 
 // The list's length of one KV head's pair of row b: its tiles, after kPairCost places for what a pair costs besides.
-constexpr int kPairCost = 2;
+constexpr int kPairCost = 5;
 template <int KT>
 __device__ __forceinline__ int pair_places(const TreeArgs& a, int len) {
   return pair_tiles<KT>(a, len) + kPairCost;
@@ -622,24 +581,47 @@ __device__ __forceinline__ void load_lds(const char* key, uint32_t key_at, const
       : "memory");
 }
 
-// Wait for all but the newest N of the wave's loads, then for the workgroup; LDS is ordered around it.
-template <int N>
-__device__ __forceinline__ void wait_barrier() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+// The same of 4 bytes a lane, or of 16 bytes a lane from one place.
+__device__ __forceinline__ void load_lds1(const char* from, uint32_t at, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(at), "s"(from) : "memory");
+}
+__device__ __forceinline__ void load_lds4(const char* from, uint32_t at, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(at), "s"(from) : "memory");
+}
+
+// Wait for all but the newest N of the wave's loads (then BARRIER: for the workgroup); LDS is ordered around it.
+template <int N, bool BARRIER>
+__device__ __forceinline__ void wait_loads() {
+  if constexpr (BARRIER) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+  else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 // All but the newest `tiles` (at most MOST) of PER loads each.
-template <int PER, int MOST>
+template <int PER, int MOST, bool BARRIER>
 __device__ __forceinline__ void wait_tiles(int tiles) {
   if constexpr (MOST > 0)
-    if (tiles < MOST) return wait_tiles<PER, MOST - 1>(tiles);
-  wait_barrier<PER * MOST>();
+    if (tiles < MOST) return wait_tiles<PER, MOST - 1, BARRIER>(tiles);
+  wait_loads<PER * MOST, BARRIER>();
 }
 // The same of LDS alone: loads stay in flight.
 __device__ __forceinline__ void lds_only_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <int E, int HD, int WQ, int WK, typename OutT>
+// A scale byte as a float, 2^(s - 127).
+__device__ __forceinline__ float scale_of(uint32_t s) { return __uint_as_float(max(s << 23, 0x00400000u)); }
+
+// Codes 0 and 1 (HIGH: 2 and 3) of four E4M3 codes times a scale, as two 16-bit numbers.  The instruction's products
+// are exact wherever the 16-bit type holds them, and rounded to nearest even elsewhere: equal to dequant2_exact's in
+// all 256 codes at all scale bytes but 255 (compared one by one), E8M0's NaN, which no quantiser stores.
+template <int E, bool HIGH>
+__device__ __forceinline__ uint32_t scaled2(uint32_t codes, float scale) {
+  if constexpr (E == kBF16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, HIGH));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, HIGH));
+}
+
+template <int E, int HD, int WQ, int WK, int TILE, bool COLD, typename OutT>
 __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_kernel(const TreeArgs a) {
-  using R = Ring<HD>;
+  using R = Ring<HD, TILE>;
   constexpr int kNW = WQ * WK, kTile = R::kTile, kRows = 32 * WQ, kStages = R::kStages;
   constexpr int kSub = kTile / (32 * WK);  // 32-position pieces of a tile that a wave takes
   constexpr int kDT = HD / 32, kKS = HD / 16;
@@ -660,10 +642,6 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qg = wave % WQ, kg = wave / WQ;
   const int l32 = lane & 31, half = lane >> 5;
-  // Of the two waves on a SIMD one multiplies while the other takes its softmax: between the barriers of a step the
-  // first four of eight waves take products, then softmax, the others the softmax of the step before, then products.
-  constexpr bool kAlternate = kNW == 8;
-  const bool behind = kAlternate && wave >= 4;
   if (id == 0)
     for (int b = tid; b < a.batch; b += 64 * kNW)
       if (a.seq_lens[b] > a.max_seq) atomicOr(a.errors, BARQ_KV_ERRBIT_ATTN_SHORT);
@@ -724,7 +702,16 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
   constexpr auto key_turn = [](int i) { return (uint32_t)((i * R::kGroup) & (HD == 64 ? 7 : 15)) << 4; };
   constexpr auto value_turn = [](int i) { return HD == 64 ? 0u : (uint32_t)((i * R::kGroup) & 3) << 6; };
   const int block_step = kTile / (int)a.div_page.d, place_step = kTile % (int)a.div_page.d;  // of a tile
-  const bool whole = (int)a.div_page.d % kPos == 0;  // a wave's positions of a tile lie in one page
+  // Cold pages: a wave takes its positions of a tile in units of two loads' groups, of which each lies in one page and
+  // has as many loads of codes and scales as of elements.  A unit's codes go to the front of its keys' (values') place
+  // in LDS, its scales 1 KB behind, and the wave decodes them where they are before the tile's step.
+  constexpr int kUnit = 2 * R::kGroup, kUnits = kPos / kUnit;
+  static_assert(!COLD || (kPos % kUnit == 0 && kUnits <= 4 && kStages <= 4), "units of a tile in four bits");
+  const int code_p = lane / (HD / 16);  // the position of a unit that a lane loads the codes of, from `code_from` on
+  const uint32_t code_from = (uint32_t)(code_p * (a.row_bytes / 2) + lane % (HD / 16) * 16);
+  uint32_t colds = 0;  // the units of the stages' tiles that hold codes
+  constexpr int kWhole = kPos < 16 ? kPos : 16;
+  const bool whole = (int)a.div_page.d % kWhole == 0;  // so many of a wave's positions of a tile lie in one page
 
   for (bool first = true; at < end;) {
     if (b >= len_row + 64) {
@@ -766,20 +753,20 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
     const auto entries = [&](int blk0) __attribute__((always_inline)) {  // a window of the block table, one entry a lane
       const int e = blk0 + lane <= last_blk ? table[blk0 + lane] : 0;
       if (e >= 0 && e < rare->num_pages) return e;
+      if (COLD && e <= -2 && -2 - e < rare->num_cold) return e;
       atomicOr(rare->errors, BARQ_KV_ERRBIT_BAD_INDEX);
       return 0;
     };
-    // The wave's block (place in it) of the next tile to load; the pages' offsets of 64 blocks from blk0 on and of
-    // the 64 after them, one a lane.
-    int blk0 = 0, blk = 0, place = 0;
-    int64_t window = 0, ahead = 0;
+    // The wave's block (place in it) of the next tile to load; the entries of 64 blocks from blk0 on and of the 64
+    // after them, one a lane.
+    int blk0 = 0, blk = 0, place = 0, window = 0, ahead = 0;
     if (count > nodes_here) {
       const int pos = c0 * kTile + wave * kPos;
       blk = (int)a.div_page.div((uint32_t)pos);
       place = pos - blk * (int)a.div_page.d;
       blk0 = min(blk, last_blk);
-      window = (int64_t)entries(blk0) * a.page_bytes;
-      ahead = (int64_t)entries(blk0 + 64) * a.page_bytes;
+      window = entries(blk0);
+      ahead = entries(blk0 + 64);
     }
     // The query has come when the table has: waited for here, and not in the loop.
 #pragma unroll
@@ -816,26 +803,66 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
     typedef __attribute__((address_space(3))) char lds_char;
     lds_char* const ring = (lds_char*)s_ring;
     const uint32_t ring_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ring);
-    const auto page_of = [&](int i) __attribute__((always_inline)) {  // a block's page, i blocks after blk0
-      const int64_t w = i < 64 ? window : ahead;
-      const uint32_t lo32 = __builtin_amdgcn_readlane((int)(uint32_t)w, i & 63);
-      const uint32_t hi32 = __builtin_amdgcn_readlane((int)(w >> 32), i & 63);
-      return (int64_t)(((uint64_t)hi32 << 32) | lo32);
+    const auto entry_of = [&](int i) __attribute__((always_inline)) {  // a block's entry, i blocks after blk0
+      return __builtin_amdgcn_readlane(i < 64 ? window : ahead, i & 63);
     };
+    const auto page_of = [&](int i) __attribute__((always_inline)) { return (int64_t)entry_of(i) * a.page_bytes; };
     const auto load_cached = [&](int t) __attribute__((always_inline)) {  // tile t of the piece; in order
       const uint32_t to = ring_at + (uint32_t)(t & (kStages - 1)) * (2 * R::kBytes) + (uint32_t)(wave * kPos * HD * 2);
       const int base = (c0 + t - nodes_here) * kTile + wave * kPos;
       if (blk >= blk0 + 64 && blk0 + 64 <= last_blk) {
         blk0 += 64;
         window = ahead;
-        ahead = (int64_t)entries(blk0 + 64) * a.page_bytes;
+        ahead = entries(blk0 + 64);
       }
-      if (whole && base + kPos <= len) {
-        const char* const k0 = kbase + (page_of(blk - blk0) + (int64_t)place * a.row_bytes);
+      if constexpr (COLD) {
+        uint32_t codes = 0;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const char* const k = k0 + (int64_t)i * R::kGroup * a.row_bytes;
-          load_lds(k, key_from ^ key_turn(i), k + to_values, value_from ^ value_turn(i), to + i * 1024, R::kBytes);
+        for (int u = 0; u < kUnits; ++u) {
+          // past the row's end: its last unit again, and in that its last position
+          const int pos = min(base + u * kUnit, (len - 1) / kUnit * kUnit), last = len - 1 - pos;
+          const int bi = (int)a.div_page.div((uint32_t)pos), off = pos - bi * (int)a.div_page.d;
+          const int e = entry_of(bi - blk0);
+          const uint32_t at = to + u * 2048;
+          if (e >= 0) {
+            const char* const k0 = kbase + ((int64_t)e * a.page_bytes + (int64_t)off * a.row_bytes);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const int back = (g * R::kGroup + min(lp, last - g * R::kGroup) - lp) * a.row_bytes;
+              const int i = 2 * u + g;
+              load_lds(k0, (key_from ^ key_turn(i)) + (uint32_t)back, k0 + to_values, (value_from ^ value_turn(i)) + (uint32_t)back,
+                       at + g * 1024, R::kBytes);
+            }
+          } else {
+            asm volatile("" : "+s"(rare));
+            const int64_t cp = -2 - (int64_t)e, p = cp * rare->page_size + off;
+            const int64_t el = p * (a.row_bytes / 2) + kvh * HD;
+            load_lds((const char*)rare->kcodes + el, code_from, (const char*)rare->vcodes + el, code_from, at, R::kBytes);
+            load_lds4((const char*)rare->kscales + (cp * a.kv_heads + kvh) * HD, (uint32_t)(lane % (HD / 16) * 16), at + 1024);
+            // a position's scale is one byte of these four (p times the heads is a multiple of 8)
+            load_lds1((const char*)rare->vscales + p * a.kv_heads, (uint32_t)((code_p * a.kv_heads + kvh) & ~3),
+                      at + 1024 + R::kBytes);
+            codes |= 1u << u;
+          }
+        }
+        const int sh = (t & (kStages - 1)) * 4;
+        colds = (colds & ~(15u << sh)) | codes << sh;
+      } else if (whole && base + kPos <= len) {
+        int at_blk = blk, at_place = place;
+#pragma unroll
+        for (int c = 0; c < kPos / kWhole; ++c) {
+          const char* const k0 = kbase + (page_of(at_blk - blk0) + (int64_t)at_place * a.row_bytes);
+#pragma unroll
+          for (int j = 0; j < kWhole / R::kGroup; ++j) {
+            const int i = c * (kWhole / R::kGroup) + j;
+            const char* const k = k0 + (int64_t)j * R::kGroup * a.row_bytes;
+            load_lds(k, key_from ^ key_turn(i), k + to_values, value_from ^ value_turn(i), to + i * 1024, R::kBytes);
+          }
+          at_place += kWhole;
+          if (at_place == (int)a.div_page.d) {
+            at_place = 0;
+            ++at_blk;
+          }
         }
       } else {
 #pragma unroll 1
@@ -854,6 +881,41 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
       if (place >= (int)a.div_page.d) {
         place -= (int)a.div_page.d;
         ++blk;
+      }
+    };
+
+    // The wave's codes of tile t, which have come, as elements in their places.
+    const auto decode = [&](int t) __attribute__((always_inline)) {
+      const uint32_t codes = colds >> (t & (kStages - 1)) * 4;
+      char* const stage = s_ring + 2 * (t & (kStages - 1)) * R::kBytes;
+#pragma unroll 1
+      for (int u = 0; u < kUnits; ++u) {
+        if (!(codes >> u & 1)) continue;
+        const int p0 = wave * kPos + u * kUnit;  // of the tile
+        char *const kp = stage + p0 * HD * 2, *const vp0 = kp + R::kBytes;
+        const int ch = lane * 4 % HD;  // a lane's four channels of keys, of positions HD / 4 lanes apart
+        uint32_t kc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kc[i] = *(const uint32_t*)(kp + lane * 4 + i * 256);
+        const uint32_t ks = *(const uint32_t*)(kp + 1024 + ch);
+        const u32x4 vc = *(const u32x4*)(vp0 + lane * 16);
+        const uint32_t vs = *(const uint32_t*)(vp0 + 1024 + lane * 4);
+        const float s0 = scale_of(ks & 255u), s1 = scale_of(ks >> 8 & 255u), s2 = scale_of(ks >> 16 & 255u), s3 = scale_of(ks >> 24);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w0 = (scaled2<E, false>(kc[i], s0) & 0xffffu) | (scaled2<E, false>(kc[i], s1) & 0xffff0000u);
+          const uint32_t w1 = (scaled2<E, true>(kc[i], s2) & 0xffffu) | (scaled2<E, true>(kc[i], s3) & 0xffff0000u);
+          *(u32x2*)(stage + key_at<HD>(p0 + (lane * 4 + i * 256) / HD, ch / 8) + (ch & 4) * 2) = u32x2{w0, w1};
+        }
+        // values past the row's end are zeros: whatever a page holds there takes no part
+        const bool in = code_p < len - (c0 + t - nodes_here) * kTile - p0;
+        const float sv = scale_of(vs >> ((code_p * a.kv_heads + kvh) & 3) * 8 & 255u);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const u32x4 w = {scaled2<E, false>(vc[2 * c], sv), scaled2<E, true>(vc[2 * c], sv),
+                           scaled2<E, false>(vc[2 * c + 1], sv), scaled2<E, true>(vc[2 * c + 1], sv)};
+          *(u32x4*)(stage + R::kBytes + value_at<HD>(p0 + code_p, lane % (HD / 16) * 2 + c)) = in ? w : u32x4{0, 0, 0, 0};
+        }
       }
     };
 
@@ -1010,10 +1072,10 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
         }
     };
 
-    // Keys of tile t are read in step t, values in step t + 1; its stage is loaded again in the step after.
-    if (!first) lds_only_barrier();  // the piece before is read from LDS
+    // A stage that step t has read is loaded again, with tile t + kStages, in the step after.
+    if (WK > 1 && !first) lds_only_barrier();  // the piece before is joined from the ring
     first = false;
-    constexpr int kAhead = kStages - 2;
+    constexpr int kAhead = kStages - 1;
     const auto load_step = [&](int t) __attribute__((always_inline)) {
       if (t + kAhead >= nodes_here && t + kAhead < count) load_cached(t + kAhead);
     };
@@ -1047,49 +1109,30 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
       load_nodes(t, false);
       load_nodes(t, true);
     }
-    wait_tiles<2 * kLoads, kAhead - 1>(min(count, kAhead) - 1);
+    const auto step_end = [&](int t) __attribute__((always_inline)) {  // tile t + 1 is there for every wave
+      wait_tiles<2 * kLoads, kAhead - 1, !COLD>(tiles_after(t));
+      if constexpr (COLD) {
+        if (t + 1 >= nodes_here && t + 1 < count) decode(t + 1);
+        lds_only_barrier();
+      }
+    };
+    step_end(-1);
     asm volatile("" : "+s"(rare));
-    const auto softmax = [&](int t) __attribute__((always_inline)) {
-      raise(t, s);
-      weights();
-    };
-    const auto step_end = [&](int t) __attribute__((always_inline)) {
-      wait_tiles<2 * kLoads, kAhead - 1>(tiles_after(t));
-    };
-    const auto products = [&](int t) __attribute__((always_inline)) {
-      __builtin_amdgcn_s_setprio(1);
-      load_step(t);
-      weigh_values(t - 1);
-      score(t);
-      __builtin_amdgcn_s_setprio(0);
-    };
     if (!wave_live) {  // no query rows: the loads alone
       for (int t = 0; t < count; ++t) {
         load_step(t);
         step_end(t);
       }
     } else {
-      load_step(0);
-      score(0);
-      if (!behind) softmax(0);
-      step_end(0);
-      if (behind) {
-        for (int t = 1; t < count; ++t) {
-          softmax(t - 1);
-          products(t);
-          step_end(t);
-        }
-        softmax(count - 1);
-      } else {
-        for (int t = 1; t < count; ++t) {
-          products(t);
-          softmax(t);
-          step_end(t);
-        }
+      for (int t = 0; t < count; ++t) {
+        load_step(t);
+        score(t);
+        raise(t, s);
+        weights();
+        weigh_values(t);
+        step_end(t);
       }
-      weigh_values(count - 1);
     }
-    if constexpr (WK > 1) lds_only_barrier();  // every wave has read the ring
     asm volatile("" : "+s"(rare));
     const f32x2 ls = halves(l);
     l = ls[0] + ls[1];
@@ -1161,10 +1204,11 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
   }
 }
 
-// Joins the records of a pair: HD / 4 threads a query row.
-template <int E, int HD, typename OutT>
+// Joins the records of a pair: HD / 4 threads a query row, which share the search for the maximum.
+template <int E, int HD, int TILE, typename OutT>
 __global__ void __launch_bounds__(kThreads) tree_flat_join_kernel(const TreeArgs a) {
-  constexpr int kPer = kThreads / (HD / 4), kTile = Ring<HD>::kTile;
+  constexpr int kLanes = HD / 4, kPer = kThreads / kLanes, kTile = TILE;
+  constexpr int kMany = 8;  // records in flight
   const int pair = (int)blockIdx.x;
   const int b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
   int before, all;
@@ -1174,32 +1218,43 @@ __global__ void __launch_bounds__(kThreads) tree_flat_join_kernel(const TreeArgs
   const int start = before * a.kv_heads + kvh * (tiles + kPairCost) + kPairCost;
   const int g0 = start / range, g1 = (start + tiles - 1) / range;
   if (g0 == g1) return;
-  const int row = (int)blockIdx.y * kPer + (int)threadIdx.x / (HD / 4);
-  const int d = ((int)threadIdx.x % (HD / 4)) * 4;
-  if (row >= a.rows) return;
-  const auto record = [&](int g) { return (int64_t)(2 * g + (g == g0)) * a.rows + row; };
-  float top = -INFINITY;
-  for (int g = g0; g <= g1; ++g) top = fmaxf(top, a.part_ml[record(g) * 2]);
-  f32x4 sum = {0, 0, 0, 0};
-  float l = 0.0f;
-#pragma unroll 4
-  for (int g = g0; g <= g1; ++g) {
-    const f32x2 ml = *(const f32x2*)(a.part_ml + record(g) * 2);
-    const f32x4 v = *(const f32x4*)(a.part + record(g) * HD + d);
-    const float by = ml[0] == -INFINITY ? 0.0f : exp2_(ml[0] - top);
-    sum += by * v;
-    l += by * ml[1];
+  const int of_row = (int)threadIdx.x % kLanes, d = of_row * 4;
+  for (int row = (int)blockIdx.y * kPer + (int)threadIdx.x / kLanes; row < a.rows; row += (int)gridDim.y * kPer) {
+    const auto record = [&](int g) { return (int64_t)(2 * g + (g == g0)) * a.rows + row; };
+    float top = -INFINITY;
+    for (int g = g0 + of_row; g <= g1; g += kLanes) top = fmaxf(top, a.part_ml[record(g) * 2]);
+#pragma unroll
+    for (int n = 1; n < kLanes; n *= 2) top = fmaxf(top, __shfl_xor(top, n, kLanes));
+    f32x4 sum = {0, 0, 0, 0};
+    float l = 0.0f;
+    for (int g = g0; g <= g1; g += kMany) {
+      f32x2 ml[kMany];
+      f32x4 v[kMany];
+#pragma unroll
+      for (int u = 0; u < kMany; ++u) {
+        const int64_t rec = record(min(g + u, g1));
+        ml[u] = *(const f32x2*)(a.part_ml + rec * 2);
+        v[u] = *(const f32x4*)(a.part + rec * HD + d);
+      }
+#pragma unroll
+      for (int u = 0; u < kMany; ++u) {
+        if (g + u > g1) break;
+        const float by = ml[u][0] == -INFINITY ? 0.0f : exp2_(ml[u][0] - top);
+        sum += by * v[u];
+        l += by * ml[u][1];
+      }
+    }
+    const float by = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const int node = (int)a.div_group.div((uint32_t)row);
+    store4<E, OutT>(a.out + (int64_t)b * a.o_sb + (int64_t)(kvh * a.group + row - node * a.group) * a.o_sh +
+                        (int64_t)node * a.o_st + d * (int)sizeof(OutT),
+                    sum * by);
   }
-  const float by = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  const int node = (int)a.div_group.div((uint32_t)row);
-  store4<E, OutT>(a.out + (int64_t)b * a.o_sb + (int64_t)(kvh * a.group + row - node * a.group) * a.o_sh +
-                      (int64_t)node * a.o_st + d * (int)sizeof(OutT),
-                  sum * by);
 }
 
 struct Plan {
   bool flat;
-  int wq, wk, tile, row_blocks, groups;
+  int wq, threads, tile, row_blocks, groups;
   int64_t splits, range, pairs, rows;
 };
 
@@ -1216,19 +1271,22 @@ bool plan_of(const barq_kv_pool* p, bool cold, int64_t batch, int64_t q_heads, i
   if (rows > (int64_t(1) << 17)) return false;
   const int64_t hd = p->head_dim, pairs_ = batch * p->kv_heads;
   // Tiles by asynchronous loads: a load's group of positions lies in one page (their offsets in 32 bits).
-  out->flat = !cold && p->page_size % (512 / hd) == 0 && p->kv_heads * hd * 2 < (int64_t(1) << 27) &&
+  out->flat = p->page_size % (cold ? 16 : 512 / hd) == 0 && p->kv_heads * hd * 2 < (int64_t(1) << 27) &&
               nodes <= (hd == 256 ? 128 : 256);  // its stages hold a tree at once
   if (out->flat) {
-    const int wq = rows > 128 && hd != 256 ? 8 : rows > 64 ? 4 : rows > 32 || hd == 256 ? 2 : 1;
-    const int64_t blocks = (rows + 32 * wq - 1) / (32 * wq), kt = hd == 256 ? 32 : 64;
+    const int wq = rows > 128 && hd != 256 && !cold ? 8 : rows > 64 ? 4 : rows > 32 ? 2 : 1;
+    const int64_t blocks = (rows + 32 * wq - 1) / (32 * wq), kt = cold ? (hd == 64 || wq <= 2 ? 128 : 64) : std::min<int64_t>(64, 8192 / hd) * (wq > 2 ? 1 : 2);
     out->wq = wq;
-    out->wk = hd == 256 || wq == 8 ? 1 : 2;
+    out->tile = (int)kt;
+    out->threads = hd == 256 ? (wq == 1 ? 128 : 256) : wq == 1 ? 256 : 512;
     out->row_blocks = (int)blocks;
     out->groups = (int)std::max<int64_t>(1, 256 / blocks);  // one workgroup a compute unit
     out->pairs = pairs_;
     out->rows = rows;
+    if (cold && hd == 256) return false;
     return pairs_ * ((longest + kt - 1) / kt + (nodes + kt - 1) / kt) < (int64_t(1) << 30);
   }
+  if (cold) return false;
   const int wq = rows > 64 ? 4 : rows > 32 || p->head_dim == 256 ? 2 : 1;
   const int tile = wq == 1 ? 128 : 64;
   const int64_t pairs = batch * p->kv_heads, blocks = (rows + 32 * wq - 1) / (32 * wq);
@@ -1254,17 +1312,15 @@ int64_t workspace_of(const Plan& p, int64_t hd) {
 }
 
 using Kernel = const void*;
-template <int E, int HD, bool COLD, typename OutT>
+template <int E, int HD, typename OutT>
 Kernel by_shape(int wq) {
   if constexpr (HD != 256)
-    if (wq == 1) return (Kernel)&tree_kernel<E, HD, 1, COLD, OutT>;
-  return wq == 2 ? (Kernel)&tree_kernel<E, HD, 2, COLD, OutT> : (Kernel)&tree_kernel<E, HD, 4, COLD, OutT>;
+    if (wq == 1) return (Kernel)&tree_kernel<E, HD, 1, OutT>;
+  return wq == 2 ? (Kernel)&tree_kernel<E, HD, 2, OutT> : (Kernel)&tree_kernel<E, HD, 4, OutT>;
 }
 template <int E, typename OutT>
-Kernel by_head(int64_t hd, bool cold, int wq) {
-  if (hd == 256) return by_shape<E, 256, false, OutT>(wq);
-  if (hd == 128) return cold ? by_shape<E, 128, true, OutT>(wq) : by_shape<E, 128, false, OutT>(wq);
-  return cold ? by_shape<E, 64, true, OutT>(wq) : by_shape<E, 64, false, OutT>(wq);
+Kernel by_head(int64_t hd, int wq) {
+  return hd == 256 ? by_shape<E, 256, OutT>(wq) : hd == 128 ? by_shape<E, 128, OutT>(wq) : by_shape<E, 64, OutT>(wq);
 }
 template <int E, typename OutT>
 Kernel join_of(int64_t hd) {
@@ -1273,26 +1329,32 @@ Kernel join_of(int64_t hd) {
                      : (Kernel)&tree_join_kernel<E, 64, OutT>;
 }
 
-template <int E, int HD, typename OutT>
+template <int E, int HD, bool COLD, typename OutT>
 Kernel flat_by_shape(const Plan& p) {
+  constexpr int kTile = COLD && HD == 64 ? 128 : 64;
   if constexpr (HD == 256) {
-    return p.wq == 4 ? (Kernel)&tree_flat_kernel<E, 256, 4, 1, OutT> : (Kernel)&tree_flat_kernel<E, 256, 2, 1, OutT>;
+    return p.wq == 4   ? (Kernel)&tree_flat_kernel<E, 256, 4, 1, 32, false, OutT>
+           : p.wq == 2 ? (Kernel)&tree_flat_kernel<E, 256, 2, 2, 64, false, OutT>
+                       : (Kernel)&tree_flat_kernel<E, 256, 1, 2, 64, false, OutT>;
   } else {
-    return p.wq == 8   ? (Kernel)&tree_flat_kernel<E, HD, 8, 1, OutT>
-           : p.wq == 4 ? (Kernel)&tree_flat_kernel<E, HD, 4, 2, OutT>
-           : p.wq == 2 ? (Kernel)&tree_flat_kernel<E, HD, 2, 2, OutT>
-                       : (Kernel)&tree_flat_kernel<E, HD, 1, 2, OutT>;
+    if constexpr (!COLD)
+      if (p.wq == 8) return (Kernel)&tree_flat_kernel<E, HD, 8, 1, kTile, false, OutT>;
+    return p.wq == 4 ? (Kernel)&tree_flat_kernel<E, HD, 4, 2, kTile, COLD, OutT>
+           : p.wq == 2 ? (Kernel)&tree_flat_kernel<E, HD, 2, 4, 128, COLD, OutT>
+                       : (Kernel)&tree_flat_kernel<E, HD, 1, 4, 128, COLD, OutT>;
   }
 }
 template <int E, typename OutT>
-Kernel flat_by_head(int64_t hd, const Plan& p) {
-  return hd == 256 ? flat_by_shape<E, 256, OutT>(p) : hd == 128 ? flat_by_shape<E, 128, OutT>(p) : flat_by_shape<E, 64, OutT>(p);
+Kernel flat_by_head(int64_t hd, bool cold, const Plan& p) {
+  if (hd == 256) return flat_by_shape<E, 256, false, OutT>(p);
+  if (hd == 128) return cold ? flat_by_shape<E, 128, true, OutT>(p) : flat_by_shape<E, 128, false, OutT>(p);
+  return cold ? flat_by_shape<E, 64, true, OutT>(p) : flat_by_shape<E, 64, false, OutT>(p);
 }
 template <int E, typename OutT>
-Kernel flat_join_of(int64_t hd) {
-  return hd == 256   ? (Kernel)&tree_flat_join_kernel<E, 256, OutT>
-         : hd == 128 ? (Kernel)&tree_flat_join_kernel<E, 128, OutT>
-                     : (Kernel)&tree_flat_join_kernel<E, 64, OutT>;
+Kernel flat_join_of(int64_t hd, const Plan& p) {
+  if (hd == 256) return p.tile == 32 ? (Kernel)&tree_flat_join_kernel<E, 256, 32, OutT> : (Kernel)&tree_flat_join_kernel<E, 256, 64, OutT>;
+  if (hd == 128) return p.tile == 64 ? (Kernel)&tree_flat_join_kernel<E, 128, 64, OutT> : (Kernel)&tree_flat_join_kernel<E, 128, 128, OutT>;
+  return p.tile == 64 ? (Kernel)&tree_flat_join_kernel<E, 64, 64, OutT> : (Kernel)&tree_flat_join_kernel<E, 64, 128, OutT>;
 }
 
 int launch(Kernel kernel, dim3 grid, void** args, void* stream, int threads = kThreads) {
@@ -1338,8 +1400,8 @@ int barq_tree_attention(const barq_kv_pool* pool, const barq_kv_cold* cold, cons
   if (cold && (hd == 256 || pool->page_size % 16 || !cold->key_codes || !cold->value_codes || !cold->key_scales ||
                !cold->value_scales || cold->num_cold < 1 || cold->num_cold >= kI32Max - 2 ||
                cold->element_type != (f16 ? BARQ_KV_FP16 : BARQ_KV_BF16) ||
-               (((uintptr_t)cold->key_codes | (uintptr_t)cold->value_codes | (uintptr_t)cold->key_scales |
-                 (uintptr_t)cold->value_scales) & 7)))
+               (((uintptr_t)cold->key_codes | (uintptr_t)cold->value_codes | (uintptr_t)cold->key_scales) & 15) ||
+               ((uintptr_t)cold->value_scales & 3)))
     return BARQ_KV_ERR_INVALID;
   const int64_t need = workspace_of(plan, hd);
   if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return BARQ_KV_ERR_INVALID;
@@ -1390,19 +1452,21 @@ int barq_tree_attention(const barq_kv_pool* pool, const barq_kv_cold* cold, cons
     a.num_cold = (int32_t)cold->num_cold;
   }
   if (plan.flat) {
-    const Kernel flat = f16 ? (f32 ? flat_by_head<kF16, float>(hd, plan) : flat_by_head<kF16, uint16_t>(hd, plan))
-                            : (f32 ? flat_by_head<kBF16, float>(hd, plan) : flat_by_head<kBF16, uint16_t>(hd, plan));
-    const Kernel join = f16 ? (f32 ? flat_join_of<kF16, float>(hd) : flat_join_of<kF16, uint16_t>(hd))
-                            : (f32 ? flat_join_of<kBF16, float>(hd) : flat_join_of<kBF16, uint16_t>(hd));
+    const Kernel flat = f16 ? (f32 ? flat_by_head<kF16, float>(hd, cold, plan) : flat_by_head<kF16, uint16_t>(hd, cold, plan))
+                            : (f32 ? flat_by_head<kBF16, float>(hd, cold, plan) : flat_by_head<kBF16, uint16_t>(hd, cold, plan));
+    const Kernel join = f16 ? (f32 ? flat_join_of<kF16, float>(hd, plan) : flat_join_of<kF16, uint16_t>(hd, plan))
+                            : (f32 ? flat_join_of<kBF16, float>(hd, plan) : flat_join_of<kBF16, uint16_t>(hd, plan));
     void* args[] = {&a};
     const int64_t per = kThreads / (hd / 4);
     const int rc = launch(flat, dim3((uint32_t)((plan.groups + 7) / 8 * 8 * plan.row_blocks)), args, stream,
-                          64 * plan.wq * plan.wk);
+                          plan.threads);
     if (rc != BARQ_KV_OK) return rc;
-    return launch(join, dim3((uint32_t)plan.pairs, (uint32_t)((plan.rows + per - 1) / per)), args, stream);
+    // Workgroups to fill the GPU once, each with the pair's place in the list found once.
+    const int64_t most = std::max<int64_t>(1, 2048 / plan.pairs);
+    return launch(join, dim3((uint32_t)plan.pairs, (uint32_t)std::min(most, (plan.rows + per - 1) / per)), args, stream);
   }
-  const Kernel kernel = f16 ? (f32 ? by_head<kF16, float>(hd, cold, plan.wq) : by_head<kF16, uint16_t>(hd, cold, plan.wq))
-                            : (f32 ? by_head<kBF16, float>(hd, cold, plan.wq) : by_head<kBF16, uint16_t>(hd, cold, plan.wq));
+  const Kernel kernel = f16 ? (f32 ? by_head<kF16, float>(hd, plan.wq) : by_head<kF16, uint16_t>(hd, plan.wq))
+                            : (f32 ? by_head<kBF16, float>(hd, plan.wq) : by_head<kBF16, uint16_t>(hd, plan.wq));
   void* args[] = {&a};
   int rc = launch(kernel, dim3((uint32_t)((a.units + 7) / 8 * 8 * plan.row_blocks)), args, stream);
   if (rc == BARQ_KV_OK && plan.splits > 1) {
