@@ -1270,10 +1270,18 @@ bool plan_of(const barq_kv_pool* p, bool cold, int64_t batch, int64_t q_heads, i
   const int64_t rows = q_heads / p->kv_heads * nodes;
   if (rows > (int64_t(1) << 17)) return false;
   const int64_t hd = p->head_dim, pairs_ = batch * p->kv_heads;
-  // Tiles by asynchronous loads: a load's group of positions lies in one page (their offsets in 32 bits).
-  out->flat = p->page_size % (cold ? 16 : 512 / hd) == 0 && p->kv_heads * hd * 2 < (int64_t(1) << 27) &&
-              nodes <= (hd == 256 ? 128 : 256);  // its stages hold a tree at once
+  // The flat list wants tiles by asynchronous loads (a load's group of positions in one page, their offsets in 32
+  // bits, a tree in its stages at once) and enough work to pay for finding each workgroup's place in it.  Whole calls,
+  // pairs cut evenly by the host -> flat list, 8 KV heads of 128, 4 query rows: 1 x 333 positions 13.2 -> 13.5 us,
+  // 16 x 333 13.6 -> 19.0, 4 x 2,900 23.6 -> 20.1, 16 x 2,900 42.6 -> 40.2; 192 query rows: 1 x 700 15.1 -> 21.8,
+  // 16 x 2,900 91.6 -> 76.7.  fp8 pages are decoded by the flat list's loads alone.
+  const int64_t mean_tiles = (std::min(mean_seq ? mean_seq : longest, longest) + 63) / 64 + (nodes + 63) / 64;
+  out->flat = (cold || pairs_ * mean_tiles > 512) && p->page_size % (cold ? 16 : 512 / hd) == 0 &&
+              p->kv_heads * hd * 2 < (int64_t(1) << 27) && nodes <= (hd == 256 ? 128 : 256);
   if (out->flat) {
+    // Groups of 32 query rows of a workgroup, and by how many positions of a tile it is cut besides: eight waves,
+    // two a SIMD, since one alone issues a vector instruction only every eighth cycle.  (fp8 pages on eight groups
+    // spill 27 registers.)
     const int wq = rows > 128 && hd != 256 && !cold ? 8 : rows > 64 ? 4 : rows > 32 ? 2 : 1;
     const int64_t blocks = (rows + 32 * wq - 1) / (32 * wq), kt = cold ? (hd == 64 || wq <= 2 ? 128 : 64) : std::min<int64_t>(64, 8192 / hd) * (wq > 2 ? 1 : 2);
     out->wq = wq;
@@ -1284,7 +1292,7 @@ bool plan_of(const barq_kv_pool* p, bool cold, int64_t batch, int64_t q_heads, i
     out->pairs = pairs_;
     out->rows = rows;
     if (cold && hd == 256) return false;
-    return pairs_ * ((longest + kt - 1) / kt + (nodes + kt - 1) / kt) < (int64_t(1) << 30);
+    return pairs_ * ((longest + kt - 1) / kt + (nodes + kt - 1) / kt + kPairCost) < (int64_t(1) << 30);
   }
   if (cold) return false;
   const int wq = rows > 64 ? 4 : rows > 32 || p->head_dim == 256 ? 2 : 1;

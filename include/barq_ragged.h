@@ -65,7 +65,8 @@ int barq_write_slots(const barq_kv_pool* pool, const int64_t* slots, const int64
  * part, whatever it holds.
  *   pool       : 2-byte elements (bf16, or fp16 with BARQ_KV_ATTN_FP16), head_dim D of 64, 128 or 256
  *   cold       : NULL, or the pool's cold store (D 64 or 128, page_size a multiple of 16, its element type
- *                the flags'): quantised blocks are read as their codes, as barq_kv_gather_cold gives them
+ *                the flags'; codes and key scales at multiples of 16 bytes): quantised blocks are read as their
+ *                codes, as barq_kv_gather_cold gives them (a scale byte of 255 is a NaN)
  *   query      : [batch, q_heads, T, D], element strides q_stride_*
  *   node_key, node_value : [batch, kv_heads, T, D], element strides node_stride_* of both
  *   mask       : bytes [batch, T, T], strides mask_stride_* (0 for what is shared), or NULL: node i sees

@@ -68,7 +68,8 @@ def test_map_slots_refusals_change_nothing(hip):
     before = [t.clone() for t in pool.tensors[2:]], pool.lens.copy(), pool.free_count
     for error, args in ((ValueError, ([1, 2], [1, 1])), (IndexError, ([1], [4])), (IndexError, ([1] * 5,)), (ValueError, ([-1],)),
                         (PagedKVCapacityError, ([20],)), (PagedKVPoolExhausted, ([0, 0, 16, 4],)),
-                        (ValueError, (torch.ones(1, dtype=torch.int64, device="cuda"),))):
+                        (ValueError, (torch.ones(1, dtype=torch.int64, device="cuda"),)),
+                        (ValueError, ([1.5],)), (ValueError, ([2], [0.5])), (ValueError, ([1 << 40 | 1, 1.0],))):
         with pytest.raises(error):
             pool.map_slots(*args)
     with pytest.raises(ValueError):
@@ -77,6 +78,8 @@ def test_map_slots_refusals_change_nothing(hip):
         map_slots_layers([pool, pool_of("cpu")], [1])
     assert all(torch.equal(a, b) for a, b in zip(before[0], pool.tensors[2:]))
     assert (pool.lens == before[1]).all() and pool.free_count == before[2]
+    for lengths in ((0, 0), np.zeros(2, dtype=np.int32), torch.zeros(2, dtype=torch.int64), [False, np.int64(0)]):
+        assert pool.map_slots(lengths).offsets.tolist() == [0, 0, 0]
     assert pool.map_slots([]).slots.numel() == 0 and pool.map_slots([0, 0]).offsets.tolist() == [0, 0, 0]
 
 

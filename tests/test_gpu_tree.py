@@ -61,27 +61,42 @@ def check(pool, q, k, v, mask, got, scale=None):
     assert pool.errors() == 0
 
 
+# Calls of little work are cut by the host, the others on the device, by the length that the call may have:
+# with a bound of `LONG` positions all are cut on the device (but where the page size or the tree does not allow it).
+LONG = 9000
+
+
+def listed_pool(listed, lens, page=16, **kw):
+    return filled(lens, page=page, extra=-(-LONG // page) if listed else 1, **kw)
+
+
+def attend(pool, listed, *args, **kw):
+    return pool.attend_tree(*args, max_seq=LONG if listed else None, **kw)
+
+
+@pytest.mark.parametrize("listed", [False, True])
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("nodes,group", [(1, 1), (1, 4), (5, 7), (13, 4), (17, 8), (64, 2), (100, 3)])
 @pytest.mark.parametrize("mask", ["chain", "shared", "rows"])
-def test_shapes(hip, dim, nodes, group, mask):
+def test_shapes(hip, dim, nodes, group, mask, listed):
     """Every head size and count of query rows, empty rows among rows that end inside tiles and pages."""
     lens = [0, 1, 63, 64, 65, 300]
-    pool = filled(lens, dim=dim, seed=nodes)
+    pool = listed_pool(listed, lens, dim=dim, seed=nodes)
     q, k, v = nodes_of(pool, len(lens), nodes, group, nodes)
     m = mask_of(mask, len(lens), nodes, nodes)
-    check(pool, q, k, v, m, pool.attend_tree(q, k, v, m))
+    check(pool, q, k, v, m, attend(pool, listed, q, k, v, m))
 
 
+@pytest.mark.parametrize("listed", [False, True])
 @pytest.mark.parametrize("page", [1, 3, 8, 16, 24, 64, 200])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-def test_pages_and_types(hip, page, dtype):
+def test_pages_and_types(hip, page, dtype, listed):
     lens = [199, 5, 128]
-    pool = filled(lens, page=page, heads=3, dim=64, dtype=dtype, seed=page)
+    pool = listed_pool(listed, lens, page=page, heads=3, dim=64, dtype=dtype, seed=page)
     q, k, v = nodes_of(pool, 3, 9, 2, page)
     m = mask_of("rows", 3, 9)
-    check(pool, q, k, v, m, pool.attend_tree(q, k, v, m))
-    got = pool.attend_tree(q, k, v, m, 0.3, out_dtype=torch.float32)
+    check(pool, q, k, v, m, attend(pool, listed, q, k, v, m))
+    got = attend(pool, listed, q, k, v, m, 0.3, out_dtype=torch.float32)
     assert got.dtype == torch.float32
     check(pool, q, k, v, m, got, 0.3)
 
@@ -99,20 +114,31 @@ def test_long_rows_are_split_and_joined(hip, dim, nodes, group, out):
     check(pool, q[:1], k[:1], v[:1], m[:1], one)
 
 
-@pytest.mark.parametrize("nodes", [128, 256])
-def test_largest_trees(hip, nodes):
-    pool = filled([70, 0], heads=1, dim=128)
-    q, k, v = nodes_of(pool, 2, nodes, 1)
-    m = mask_of("rows", 2, nodes)
-    check(pool, q, k, v, m, pool.attend_tree(q, k, v, m))
+@pytest.mark.parametrize("dim,nodes,group", [(128, 5, 4), (64, 12, 8), (256, 3, 4)])
+def test_many_rows_of_few_positions(hip, dim, nodes, group):
+    """More rows than a wave has lanes, most of them short: ranges of many pairs, and pairs of many ranges."""
+    lens = [(i * 37) % 90 for i in range(150)] + [2500]
+    pool = filled(lens, heads=3, dim=dim, seed=2)
+    q, k, v = nodes_of(pool, len(lens), nodes, group, 2)
     check(pool, q, k, v, None, pool.attend_tree(q, k, v))
 
 
+@pytest.mark.parametrize("listed", [False, True])
+@pytest.mark.parametrize("dim,nodes", [(128, 128), (128, 256), (64, 256), (256, 128), (256, 129)])
+def test_largest_trees(hip, dim, nodes, listed):
+    pool = listed_pool(listed, [70, 0], heads=4, dim=dim)
+    q, k, v = nodes_of(pool, 2, nodes, 1)
+    m = mask_of("rows", 2, nodes)
+    check(pool, q, k, v, m, attend(pool, listed, q, k, v, m))
+    check(pool, q, k, v, None, attend(pool, listed, q, k, v))
+
+
+@pytest.mark.parametrize("listed", [False, True])
 @pytest.mark.parametrize("dim,group", [(64, 1), (128, 4), (128, 8), (256, 4)])
-def test_what_a_node_does_not_see_takes_no_part(hip, dim, group):
+def test_what_a_node_does_not_see_takes_no_part(hip, dim, group, listed):
     """Infinities and NaN in nodes that others do not see, keys and values; what sees them has them."""
     nodes = 40
-    pool = filled([150, 0], dim=dim, seed=5)
+    pool = listed_pool(listed, [150, 0], dim=dim, heads=4, seed=5)
     q, k, v = nodes_of(pool, 2, nodes, group, 5)
     k, v = k.clone(), v.clone()
     m = torch.eye(nodes, dtype=torch.bool).expand(2, nodes, nodes).clone()
@@ -122,7 +148,7 @@ def test_what_a_node_does_not_see_takes_no_part(hip, dim, group):
         k[:, :, j, ::3] = x
         v[:, :, j, 1::5] = x
     clean = [i for i in range(nodes) if i not in wild]
-    got = pool.attend_tree(q, k, v, m.cuda())
+    got = attend(pool, listed, q, k, v, m.cuda())
     ko, vo = pool.gather(2, 150)
     out, weight, score = tree_reference(q, ko, vo, pool.lens, k, v, m, dim**-0.5)
     bound = tree_bound(out, weight, score, got.dtype, 200, dim)
@@ -131,7 +157,7 @@ def test_what_a_node_does_not_see_takes_no_part(hip, dim, group):
     k2, v2 = nodes_of(pool, 2, nodes, group, 6)[1:]
     v2 = v2.clone()
     v2[:, :, 20, 1::5] = math.inf
-    got = pool.attend_tree(q, k2, v2, m.cuda()).float().cpu()
+    got = attend(pool, listed, q, k2, v2, m.cuda()).float().cpu()
     assert (got[:, :, 20, 1::5] == math.inf).all()
     got[:, :, 20, 1::5] = 0
     assert got.isfinite().all()
@@ -141,44 +167,46 @@ def test_what_a_node_does_not_see_takes_no_part(hip, dim, group):
     assert (got.double() - out).abs()[:, :, rest].le(bound[:, :, rest]).all()
 
 
-def test_large_scores(hip):
+@pytest.mark.parametrize("listed", [False, True])
+def test_large_scores(hip, listed):
     """Scores of some hundreds, rising along the row, so that the running maximum moves often; and all equal."""
-    pool = filled([700], heads=1, dim=128, scale=1.0, seed=3)
+    pool = listed_pool(listed, [700], heads=5, dim=128, scale=1.0, seed=3)
     q, k, v = nodes_of(pool, 1, 6, 4, 3)
     q = q * 16
-    check(pool, q, k, v, None, pool.attend_tree(q, k, v))
+    check(pool, q, k, v, None, attend(pool, listed, q, k, v))
     zero = torch.zeros_like(q)
-    check(pool, zero, k, v, None, pool.attend_tree(zero, k, v))
+    check(pool, zero, k, v, None, attend(pool, listed, zero, k, v))
 
 
-def test_layouts_and_outputs(hip):
+@pytest.mark.parametrize("listed", [False, True])
+def test_layouts_and_outputs(hip, listed):
     """Strided and misaligned inputs, an out of the caller's, masks of any strides, fewer rows than the pool."""
     lens = [90, 31, 200]
-    pool = filled(lens, heads=2, dim=64)
+    pool = listed_pool(listed, lens, heads=2, dim=64)
     q, k, v = nodes_of(pool, 3, 10, 3, layout="heads")
     m = mask_of("rows", 3, 10)
-    want = pool.attend_tree(q, k, v, m)
+    want = attend(pool, listed, q, k, v, m)
     check(pool, q, k, v, m, want)
     flat = torch.zeros((3 * 10 * 6 * 64 + 1,), dtype=q.dtype, device="cuda")
     odd = flat[1:].view(3, 6, 10, 64).copy_(q)
     wide = torch.zeros((3, 2, 10, 65), dtype=q.dtype, device="cuda")
     wide[..., :64] = k
     turned = v.transpose(2, 3).contiguous().transpose(2, 3)
-    assert torch.equal(pool.attend_tree(odd, wide[..., :64], turned, m.transpose(1, 2).contiguous().transpose(1, 2)), want)
+    assert torch.equal(attend(pool, listed, odd, wide[..., :64], turned, m.transpose(1, 2).contiguous().transpose(1, 2)), want)
     for dtype in (q.dtype, torch.float32):
         for shape, turn in (((3, 6, 10, 64), False), ((3, 10, 6, 64), True), ((3, 6, 10, 67), False)):
             buffer = torch.full(shape, 7.0, dtype=dtype, device="cuda")
             out = buffer.transpose(1, 2) if turn else buffer[..., :64]
-            got = pool.attend_tree(q, k, v, m, out=out)
+            got = attend(pool, listed, q, k, v, m, out=out)
             assert got.data_ptr() == out.data_ptr() and torch.equal(got.to(q.dtype), want)
             assert (buffer[..., 64:] == 7).all()
-    two = pool.attend_tree(q[:2], k[:2], v[:2], m[:2])
+    two = attend(pool, listed, q[:2], k[:2], v[:2], m[:2])
     check(pool, q[:2], k[:2], v[:2], m[:2], two)
     expanded = m[:1].expand(3, 10, 10)
-    assert torch.equal(pool.attend_tree(q, k, v, expanded), pool.attend_tree(q, k, v, m[0]))
-    assert torch.equal(pool.attend_tree(q, k, v, m[:1]), pool.attend_tree(q, k, v, m[0]))
+    assert torch.equal(attend(pool, listed, q, k, v, expanded), attend(pool, listed, q, k, v, m[0]))
+    assert torch.equal(attend(pool, listed, q, k, v, m[:1]), attend(pool, listed, q, k, v, m[0]))
     one = torch.zeros((1, 2, 1, 64), dtype=q.dtype, device="cuda")  # dimensions of one: their strides do not count
-    check(pool, q[:1, :, :1], one, one, None, pool.attend_tree(q[:1, :, :1], one.as_strided((1, 2, 1, 64), (3, 64, 5, 1)), one))
+    check(pool, q[:1, :, :1], one, one, None, attend(pool, listed, q[:1, :, :1], one.as_strided((1, 2, 1, 64), (3, 64, 5, 1)), one))
 
 
 def test_refusals(hip):
@@ -259,7 +287,7 @@ def test_streams_and_captured_replays(hip):
 
 
 def test_the_same_call_gives_the_same_bits(hip):
-    pool = filled([2000, 100, 700], dim=128, heads=4)
+    pool = filled([2000, 100, 7000], dim=128, heads=4)
     q, k, v = nodes_of(pool, 3, 24, 4)
     m = mask_of("rows", 3, 24)
     first = pool.attend_tree(q, k, v, m)
@@ -269,6 +297,7 @@ def test_the_same_call_gives_the_same_bits(hip):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("dim,page,nodes,group", [(128, 16, 6, 4), (64, 32, 20, 3), (128, 48, 70, 2), (64, 16, 1, 1),
+                                                  (64, 16, 33, 4), (128, 32, 40, 4), (128, 16, 9, 4),
                                                   (64, 8, 5, 2), (256, 16, 5, 2)])
 def test_fp8_pages(hip, dtype, dim, page, nodes, group):
     """Quantised blocks as the dequantising gather gives them; page sizes and heads the kernel does not decode too."""

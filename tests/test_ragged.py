@@ -164,7 +164,8 @@ def test_map_slots_refusals_change_nothing():
     cases = [
         (ValueError, dict(lengths=[1, 2], rows=[0])), (ValueError, dict(lengths=[1, 2], rows=[1, 1])),
         (IndexError, dict(lengths=[1], rows=[4])), (IndexError, dict(lengths=[1], rows=[-1])),
-        (IndexError, dict(lengths=[1] * 5)), (ValueError, dict(lengths=[-1])), (ValueError, dict(lengths=np.array([1.5]))), (ValueError, dict(lengths=torch.ones((1, 1), dtype=torch.int64))),
+        (IndexError, dict(lengths=[1] * 5)), (ValueError, dict(lengths=[-1])), (ValueError, dict(lengths=np.array([1.5]))),
+        (ValueError, dict(lengths=[1.5])), (ValueError, dict(lengths=[2], rows=[0.5])), (ValueError, dict(lengths=torch.ones((1, 1), dtype=torch.int64))),
         (PagedKVCapacityError, dict(lengths=[20])), (PagedKVCapacityError, dict(lengths=[4], max_length=8)),
         (PagedKVPoolExhausted, dict(lengths=[0, 0, 16, 4])),
     ]
