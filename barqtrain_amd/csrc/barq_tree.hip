@@ -5,12 +5,13 @@
 //   tensors), h of KV head h / G.
 //
 // Split.  The G * T query rows of a (row, KV head) pair share every key and value, so a workgroup takes a block of
-// 32 * WQ of them and a range of the pair's tiles of positions: the cached ones, then the nodes.  Its four waves
-// are WQ groups of 32 query rows by WK = 4 / WQ groups of a tile's positions.  Ranges of one pair are joined by a
-// second launch from their unnormalised sums, maxima and sums (32 bits), or the one range writes the output.
-//
-// A tile's keys and values go through registers into LDS, the next tile's loads in flight while this one is
-// computed, the block table's entries one tile further ahead.
+// 32 * WQ of them and a range of the pair's tiles of positions: the cached ones and the nodes.  Its waves are WQ
+// groups of 32 query rows by WK groups of a tile's positions.  Ranges of one pair are joined by a second launch from
+// their unnormalised sums, maxima and sums (32 bits), or the one range writes the output.  Two kernels:
+//   tree_kernel       little work, page sizes and trees that the other does not take: the host cuts each pair into
+//                     equal ranges; tiles go through registers into LDS, the next one's loads in flight while this
+//                     one is computed, the block table's entries one tile further ahead.
+//   tree_flat_kernel  the rest, and fp8 pages: the device cuts the list of all pairs' tiles; tiles go straight to LDS.
 //
 // Arithmetic.  S^T = K Q^T and O^T = V^T P^T on the 32x32x16 MFMA, so that a lane holds 16 positions' scores of ONE
 // query row: the softmax needs no lane exchange but with lane ^ 32, and the lane's scores are, as they stand, its
@@ -20,6 +21,12 @@
 // the rounded value and the rounded remainder (2^-17 of the value is lost in bf16): one alone would add an error
 // as large as the output's own rounding.  Running maximum and sum per query row in base 2, 32 bits; the sums are
 // rescaled only when a maximum grows by more than 2^8, which every exponent here holds.
+//
+// What bounds it.  Few query rows: the pages' bytes.  From about 64 query rows a pair the matrix units: with the
+// remainders' product a key costs 1.5 times the two products' operations.  64 nodes of 8 heads a KV head over 32 rows
+// of up to 4,096 positions run at 960 TFLOP/s, three quarters of what one large product reaches on the card; deeper
+// prefetch, another order of products and softmax, wave priorities and other batches of reads changed that by 2% at
+// most, and the remainders' share is the price of errors as small as the rounding of the output.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -529,6 +536,14 @@ __global__ void __launch_bounds__(kThreads) tree_join_kernel(const TreeArgs a, i
 // one list; group g of row_blocks workgroups takes the g-th equal range of it, whatever the rows' lengths.
 // A range's piece of a pair that is not the whole pair leaves a record (slot 2g for a piece that begins inside its
 // pair, else 2g + 1: a range has at most one of each), joined by a second launch in the order of the groups.
+//
+// A tile's keys and values go to LDS by asynchronous loads, 128 KB of them: the stages but one are in flight while
+// one is computed.  Each step a wave waits for its own loads of the next
+// tile, decodes what codes it loaded, and meets the others at one barrier; nothing else waits for memory.
+// Whole calls, host's cut and tiles through registers -> this (us; 8 KV heads of 128): 16 rows of 512 to 2,048
+// positions, 24 nodes x 4 query heads 53.6 -> 39.6; one row of 32,749, 64 x 4 95.9 -> 77.0; 32 rows of 512 to 4,096,
+// 64 x 8 355 -> 265; 4 heads of 256, 12 rows of 1,500, 7 x 2 31.4 -> 27.7; 16 rows of 2,000, fp8 pages, 16 x 4
+// 96.1 -> 43.0.
 template <int HD, int TILE>
 struct Ring {
   static constexpr int kTile = TILE;                 // positions of a tile
@@ -545,7 +560,9 @@ __device__ __forceinline__ int pair_tiles(const TreeArgs& a, int len) {
   return (len + KT - 1) / KT + (a.nodes + KT - 1) / KT;
 }
 
-// The list's length of one KV head's pair of row b: its tiles, after kPairCost places for what a pair costs besides.
+// The list's length of one KV head's pair of row b: its tiles, after kPairCost places for what a pair costs besides
+// (query, table, mask, nodes, record: 9 to 12 us with 256 query rows, where a tile takes 2.3).  With 2 places the workgroup with a row of
+// no positions took 283 us where the average took 190; with 5 all 32 rows take 250; 4, 6 and 8 within 2%.
 constexpr int kPairCost = 5;
 template <int KT>
 __device__ __forceinline__ int pair_places(const TreeArgs& a, int len) {
@@ -710,7 +727,8 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
   const int code_p = lane / (HD / 16);  // the position of a unit that a lane loads the codes of, from `code_from` on
   const uint32_t code_from = (uint32_t)(code_p * (a.row_bytes / 2) + lane % (HD / 16) * 16);
   uint32_t colds = 0;  // the units of the stages' tiles that hold codes
-  constexpr int kWhole = kPos < 16 ? kPos : 16;
+  constexpr int kWhole = 8;
+  static_assert(kPos % kWhole == 0 && kWhole % R::kGroup == 0, "whole parts of a wave's positions");
   const bool whole = (int)a.div_page.d % kWhole == 0;  // so many of a wave's positions of a tile lie in one page
 
   for (bool first = true; at < end;) {
@@ -830,15 +848,16 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
             for (int g = 0; g < 2; ++g) {
               const int back = (g * R::kGroup + min(lp, last - g * R::kGroup) - lp) * a.row_bytes;
               const int i = 2 * u + g;
-              load_lds(k0, (key_from ^ key_turn(i)) + (uint32_t)back, k0 + to_values, (value_from ^ value_turn(i)) + (uint32_t)back,
-                       at + g * 1024, R::kBytes);
+              load_lds(k0, (key_from ^ key_turn(i)) + (uint32_t)back, k0 + to_values,
+                       (value_from ^ value_turn(i)) + (uint32_t)back, at + g * 1024, R::kBytes);
             }
           } else {
             asm volatile("" : "+s"(rare));
             const int64_t cp = -2 - (int64_t)e, p = cp * rare->page_size + off;
             const int64_t el = p * (a.row_bytes / 2) + kvh * HD;
             load_lds((const char*)rare->kcodes + el, code_from, (const char*)rare->vcodes + el, code_from, at, R::kBytes);
-            load_lds4((const char*)rare->kscales + (cp * a.kv_heads + kvh) * HD, (uint32_t)(lane % (HD / 16) * 16), at + 1024);
+            load_lds4((const char*)rare->kscales + (cp * a.kv_heads + kvh) * HD, (uint32_t)(lane % (HD / 16) * 16),
+                      at + 1024);
             // a position's scale is one byte of these four (p times the heads is a multiple of 8)
             load_lds1((const char*)rare->vscales + p * a.kv_heads, (uint32_t)((code_p * a.kv_heads + kvh) & ~3),
                       at + 1024 + R::kBytes);
@@ -872,8 +891,8 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
           const int bi = (int)a.div_page.div((uint32_t)pos);
           const char* const k = kbase + (page_of(bi - blk0) + (int64_t)(pos - bi * (int)a.div_page.d) * a.row_bytes);
           const uint32_t back = (uint32_t)(max(lp - (len - 1 - pos), 0) * a.row_bytes);
-          load_lds(k, (key_from ^ ((uint32_t)((i * R::kGroup) & (HD == 64 ? 7 : 15)) << 4)) - back, k + to_values,
-                   (value_from ^ (HD == 64 ? 0u : (uint32_t)((i * R::kGroup) & 3) << 6)) - back, to + i * 1024, R::kBytes);
+          load_lds(k, (key_from ^ key_turn(i)) - back, k + to_values, (value_from ^ value_turn(i)) - back, to + i * 1024,
+                   R::kBytes);
         }
       }
       blk += block_step;
@@ -900,7 +919,8 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
         const uint32_t ks = *(const uint32_t*)(kp + 1024 + ch);
         const u32x4 vc = *(const u32x4*)(vp0 + lane * 16);
         const uint32_t vs = *(const uint32_t*)(vp0 + 1024 + lane * 4);
-        const float s0 = scale_of(ks & 255u), s1 = scale_of(ks >> 8 & 255u), s2 = scale_of(ks >> 16 & 255u), s3 = scale_of(ks >> 24);
+        const float s0 = scale_of(ks & 255u), s1 = scale_of(ks >> 8 & 255u);
+        const float s2 = scale_of(ks >> 16 & 255u), s3 = scale_of(ks >> 24);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t w0 = (scaled2<E, false>(kc[i], s0) & 0xffffu) | (scaled2<E, false>(kc[i], s1) & 0xffff0000u);
@@ -925,15 +945,18 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
     for (int d = 0; d < kDT; ++d) o[d] = f32x16{0};
     float m = -INFINITY, l = 0.0f;
 
+    const auto turned = [](const lds_char* p, uint32_t bits) __attribute__((always_inline)) {
+      return (lds_char*)(uintptr_t)((uint32_t)(uintptr_t)p ^ bits);
+    };
     u32x4 key[2][kKeys];
     const auto read_keys = [&](const lds_char* from, int n, u32x4 (&to)[kKeys]) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < kKeys; ++i) {
         const int u = (n * kKeys + i) / kKS, k = (n * kKeys + i) % kKS;
-        to[i] = *(const __attribute__((address_space(3))) u32x4*)((const lds_char*)(uintptr_t)((uint32_t)(uintptr_t)from ^ (uint32_t)(k << 5)) + u * 32 * HD * 2);
+        const lds_char* const at = turned(from, (uint32_t)(k << 5)) + u * 32 * HD * 2;
+        to[i] = *(const __attribute__((address_space(3))) u32x4*)at;
       }
     };
-    const auto key_stage = [&](int t) __attribute__((always_inline)) { return ring + (t & (kStages - 1)) * (2 * R::kBytes) + key_lane; };
     constexpr int kKeyBatches = kSub * kKS / kKeys;
 
     // ---- V of tile t times its probabilities
@@ -946,7 +969,7 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
 #pragma unroll
         for (int i = 0; i < kVals; ++i) {
           const int d = n % (kDT / kVals) * kVals + i;
-          lds_char* const x = (lds_char*)(uintptr_t)((uint32_t)(uintptr_t)from ^ (uint32_t)(d << 6)) + n / (kDT / kVals) * 16 * HD * 2;
+          lds_char* const x = turned(from, (uint32_t)(d << 6)) + n / (kDT / kVals) * 16 * HD * 2;
           const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)x);
           const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(x + 8 * HD * 2));
           const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
@@ -1040,7 +1063,7 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
 
     // ---- scores of tile t
     const auto score = [&](int t) __attribute__((always_inline)) {
-      const lds_char* const keys = key_stage(t);
+      const lds_char* const keys = ring + (t & (kStages - 1)) * (2 * R::kBytes) + key_lane;
       read_keys(keys, 0, key[0]);
 #pragma unroll
       for (int u = 0; u < kSub; ++u) s[u] = f32x16{0};
@@ -1081,7 +1104,9 @@ __global__ void __launch_bounds__(64 * WQ * WK, WQ * WK == 8 ? 2 : 1) tree_flat_
     };
     for (int t = nodes_here; t < min(count, kAhead); ++t) load_cached(t);
     // tiles on their way when step t + 1 needs its own
-    const auto tiles_after = [&](int t) __attribute__((always_inline)) { return max(min(count - 1, t + kAhead) - (t + 1), 0); };
+    const auto tiles_after = [&](int t) __attribute__((always_inline)) {
+      return max(min(count - 1, t + kAhead) - (t + 1), 0);
+    };
     if (nodes_here > 0) {  // the tree's mask as bits
       if (tid < kWords) s_bad[tid] = 0;
       const int rows_here = (int)a.div_group.div((uint32_t)min(rb * kRows + kRows - 1, rare->rows - 1)) - node_lo + 1;
@@ -1269,40 +1294,47 @@ bool plan_of(const barq_kv_pool* p, bool cold, int64_t batch, int64_t q_heads, i
   const int64_t longest = max_seq == 0 ? cap : std::min(max_seq, cap);
   const int64_t rows = q_heads / p->kv_heads * nodes;
   if (rows > (int64_t(1) << 17)) return false;
-  const int64_t hd = p->head_dim, pairs_ = batch * p->kv_heads;
+  const int64_t hd = p->head_dim, pairs = batch * p->kv_heads;
   // The flat list wants tiles by asynchronous loads (a load's group of positions in one page, their offsets in 32
   // bits, a tree in its stages at once) and enough work to pay for finding each workgroup's place in it.  Whole calls,
   // pairs cut evenly by the host -> flat list, 8 KV heads of 128, 4 query rows: 1 x 333 positions 13.2 -> 13.5 us,
   // 16 x 333 13.6 -> 19.0, 4 x 2,900 23.6 -> 20.1, 16 x 2,900 42.6 -> 40.2; 192 query rows: 1 x 700 15.1 -> 21.8,
   // 16 x 2,900 91.6 -> 76.7.  fp8 pages are decoded by the flat list's loads alone.
   const int64_t mean_tiles = (std::min(mean_seq ? mean_seq : longest, longest) + 63) / 64 + (nodes + 63) / 64;
-  out->flat = (cold || pairs_ * mean_tiles > 512) && p->page_size % (cold ? 16 : 512 / hd) == 0 &&
+  if (cold && hd == 256) return false;
+  out->flat = (cold || pairs * mean_tiles > 512) && p->page_size % (cold ? 16 : 512 / hd) == 0 &&
               p->kv_heads * hd * 2 < (int64_t(1) << 27) && nodes <= (hd == 256 ? 128 : 256);
   if (out->flat) {
     // Groups of 32 query rows of a workgroup, and by how many positions of a tile it is cut besides: eight waves,
     // two a SIMD, since one alone issues a vector instruction only every eighth cycle.  (fp8 pages on eight groups
     // spill 27 registers.)
     const int wq = rows > 128 && hd != 256 && !cold ? 8 : rows > 64 ? 4 : rows > 32 ? 2 : 1;
-    const int64_t blocks = (rows + 32 * wq - 1) / (32 * wq), kt = cold ? (hd == 64 || wq <= 2 ? 128 : 64) : std::min<int64_t>(64, 8192 / hd) * (wq > 2 ? 1 : 2);
+    const int64_t blocks = (rows + 32 * wq - 1) / (32 * wq);
+    // 64 positions a tile (32 of head size 256), twice as many with few query rows: a 32-position piece for every
+    // wave.  fp8 pages of head size 64 take 128 always, since a load of codes covers 16 of them.
+    const int64_t kt = cold && hd == 64 ? 128 : std::min<int64_t>(64, 8192 / hd) * (wq > 2 ? 1 : 2);
     out->wq = wq;
     out->tile = (int)kt;
     out->threads = hd == 256 ? (wq == 1 ? 128 : 256) : wq == 1 ? 256 : 512;
     out->row_blocks = (int)blocks;
     out->groups = (int)std::max<int64_t>(1, 256 / blocks);  // one workgroup a compute unit
-    out->pairs = pairs_;
+    out->pairs = pairs;
     out->rows = rows;
-    if (cold && hd == 256) return false;
-    return pairs_ * ((longest + kt - 1) / kt + (nodes + kt - 1) / kt + kPairCost) < (int64_t(1) << 30);
+    return pairs * ((longest + kt - 1) / kt + (nodes + kt - 1) / kt + kPairCost) < (int64_t(1) << 30);
   }
   if (cold) return false;
   const int wq = rows > 64 ? 4 : rows > 32 || p->head_dim == 256 ? 2 : 1;
   const int tile = wq == 1 ? 128 : 64;
-  const int64_t pairs = batch * p->kv_heads, blocks = (rows + 32 * wq - 1) / (32 * wq);
+  const int64_t blocks = (rows + 32 * wq - 1) / (32 * wq);
   const auto tiles_of = [&](int64_t n) { return (n + tile - 1) / tile + (nodes + tile - 1) / tile; };
   const int64_t most = tiles_of(longest), mean = tiles_of(mean_seq ? std::min(mean_seq, longest) : longest);
   const int64_t want = p->head_dim == 256 ? 256 : 512;  // workgroups that are resident at once
-  // A range keeps two tiles at least; mean tiles a pair over all of the launch's ranges.
-  int64_t range = std::max<int64_t>(2, (mean * pairs * blocks + want - 1) / want);
+  // The mean tiles of a pair over all of the launch's ranges; two tiles a range at least, since a join costs what a
+  // tile does, but one of the 128 positions of few query rows where a pair is cut anyhow.  Whole calls, two -> one (us):
+  // 4 query rows of head size 128 over 333 / 700 / 1,500 positions 13.5 / 13.6 / 14.6 -> 11.3 / 12.3 / 13.2, over 100
+  // (two tiles) 10.6 -> 11.5; 52 query rows over 1,500 14.6 -> 15.9.
+  const int64_t least = wq == 1 && most > 2 ? 1 : 2;
+  int64_t range = std::max<int64_t>(least, (mean * pairs * blocks + want - 1) / want);
   range = std::min(range, most);
   out->wq = wq;
   out->tile = tile;
@@ -1360,8 +1392,10 @@ Kernel flat_by_head(int64_t hd, bool cold, const Plan& p) {
 }
 template <int E, typename OutT>
 Kernel flat_join_of(int64_t hd, const Plan& p) {
-  if (hd == 256) return p.tile == 32 ? (Kernel)&tree_flat_join_kernel<E, 256, 32, OutT> : (Kernel)&tree_flat_join_kernel<E, 256, 64, OutT>;
-  if (hd == 128) return p.tile == 64 ? (Kernel)&tree_flat_join_kernel<E, 128, 64, OutT> : (Kernel)&tree_flat_join_kernel<E, 128, 128, OutT>;
+  if (hd == 256)
+    return p.tile == 32 ? (Kernel)&tree_flat_join_kernel<E, 256, 32, OutT> : (Kernel)&tree_flat_join_kernel<E, 256, 64, OutT>;
+  if (hd == 128)
+    return p.tile == 64 ? (Kernel)&tree_flat_join_kernel<E, 128, 64, OutT> : (Kernel)&tree_flat_join_kernel<E, 128, 128, OutT>;
   return p.tile == 64 ? (Kernel)&tree_flat_join_kernel<E, 64, 64, OutT> : (Kernel)&tree_flat_join_kernel<E, 64, 128, OutT>;
 }
 

@@ -370,7 +370,8 @@ class PagePool:
     def write_slots(self, slots: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                     index: Optional[torch.Tensor] = None) -> None:
         """Store token ``index[j]`` (default: j) of ``key`` / ``value`` ``[tokens, kv_heads, head_dim]`` in slot
-        ``slots[j]`` (int64, as `map_slots` gives them; negative ones are passed over).  The accepted nodes of
+        ``slots[j]`` (int64, as `map_slots` gives them; negative ones are passed over; a slot named twice ends with pieces
+        of either token).  The accepted nodes of
         drafted trees ``[batch, kv_heads, nodes, head_dim]`` are ``states.transpose(1, 2).flatten(0, 1)`` with
         ``index`` = row * nodes + node."""
         if self.on_gpu:

@@ -88,11 +88,12 @@ def test_shapes(hip, dim, nodes, group, mask, listed):
 
 
 @pytest.mark.parametrize("listed", [False, True])
-@pytest.mark.parametrize("page", [1, 3, 8, 16, 24, 64, 200])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [1, 3, 4, 8, 16, 24, 64, 200])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-def test_pages_and_types(hip, page, dtype, listed):
+def test_pages_and_types(hip, page, dtype, dim, listed):
     lens = [199, 5, 128]
-    pool = listed_pool(listed, lens, page=page, heads=3, dim=64, dtype=dtype, seed=page)
+    pool = listed_pool(listed, lens, page=page, heads=3, dim=dim, dtype=dtype, seed=page)
     q, k, v = nodes_of(pool, 3, 9, 2, page)
     m = mask_of("rows", 3, 9)
     check(pool, q, k, v, m, attend(pool, listed, q, k, v, m))
@@ -228,10 +229,12 @@ def test_refusals(hip):
         with pytest.raises(ValueError):
             other.attend_tree(x, x, x)
     assert pool.attend_tree(q[:, :, :0], k[:, :, :0], v[:, :, :0]).shape == (1, 4, 0, 64)
+    assert pool.attend_tree(q[:0], k[:0], v[:0]).shape == (0, 4, 3, 64)
 
 
-def test_rows_longer_than_max_seq_and_bad_pages_are_flagged(hip):
-    pool = filled([100, 40], dim=64)
+@pytest.mark.parametrize("heads", [2, 130])
+def test_rows_longer_than_max_seq_and_bad_pages_are_flagged(hip, heads):
+    pool = filled([100, 40], dim=64, heads=heads)
     q, k, v = nodes_of(pool, 2, 4, 2)
     got = pool.attend_tree(q, k, v, max_seq=50)
     assert pool.errors() == 16  # BARQ_KV_ERRBIT_ATTN_SHORT
@@ -246,19 +249,21 @@ def test_rows_longer_than_max_seq_and_bad_pages_are_flagged(hip):
     assert pool.errors() == 4  # BARQ_KV_ERRBIT_BAD_INDEX
 
 
-def test_page_offsets_past_32_bits(hip):
+@pytest.mark.parametrize("blocks", [8, 600])
+def test_page_offsets_past_32_bits(hip, blocks):
     pages = 140000  # 4.6 GB of keys
-    pool = PagePool(max_batch=1, max_blocks=8, page_size=16, kv_heads=8, head_dim=128, dtype=torch.bfloat16, device="cuda",
+    pool = PagePool(max_batch=1, max_blocks=blocks, page_size=16, kv_heads=8, head_dim=128, dtype=torch.bfloat16, device="cuda",
                     num_pages=pages, page_order=torch.arange(pages - 1, -1, -1))
     g = torch.Generator().manual_seed(0)
     pool.append(*(torch.randn((1, 8, 77, 128), generator=g).to(torch.bfloat16).cuda() for _ in range(2)))
     q, k, v = nodes_of(pool, 1, 4, 2)
-    check(pool, q, k, v, None, pool.attend_tree(q, k, v))
+    check(pool, q, k, v, None, pool.attend_tree(q, k, v, max_seq=pool.capacity))
 
 
-def test_streams_and_captured_replays(hip):
+@pytest.mark.parametrize("extra", [8, 600])
+def test_streams_and_captured_replays(hip, extra):
     """Two captured graphs of one pool and eager calls between their replays; rows grow between replays."""
-    pool = filled([300, 10], dim=128, heads=2, extra=8)
+    pool = filled([300, 10], dim=128, heads=2, extra=extra)
     inputs = [nodes_of(pool, 2, n, 4, n) for n in (5, 20)]
     masks = [mask_of("rows", 2, n, n) for n in (5, 20)]
     graphs, outs = [], []
