@@ -616,15 +616,19 @@ bool crop_layers_(const std::vector<at::Tensor>& seq_lens, const std::vector<py:
   return true;
 }
 
-// Reset of a model's pools, packed by pool_group and (all of them or none) cold_group, in one launch; like: a tensor of theirs (device, stream).
+// Reset of a model's pools, packed by pool_group (one or several a group) and, all of them or none and one a group,
+// cold_group, in one launch; like: a tensor of theirs (device, stream).
 void reset_layers_(const std::vector<at::Tensor>& pools, const std::vector<at::Tensor>& colds, const at::Tensor& like) {
   TORCH_CHECK(like.is_cuda() && (colds.empty() || colds.size() == pools.size()), "reset_layers_: one cold store per pool");
   std::vector<barq_kv_pool> ps;
   std::vector<barq_kv_cold> cs;
   for (const at::Tensor& t : pools) {
-    TORCH_CHECK(t.device().is_cpu() && t.scalar_type() == at::kByte && t.numel() == (int64_t)sizeof(barq_kv_pool),
-                "not a one-pool group (see pool_group)");
-    ps.push_back(*reinterpret_cast<const barq_kv_pool*>(t.data_ptr<uint8_t>()));
+    const int64_t n = t.numel() / (int64_t)sizeof(barq_kv_pool);
+    TORCH_CHECK(t.device().is_cpu() && t.scalar_type() == at::kByte && t.is_contiguous() && n > 0 &&
+                    t.numel() == n * (int64_t)sizeof(barq_kv_pool) && (n == 1 || colds.empty()),
+                "not a pool group, or with cold stores a one-pool group (see pool_group)");
+    const auto* p = reinterpret_cast<const barq_kv_pool*>(t.data_ptr<uint8_t>());
+    ps.insert(ps.end(), p, p + n);
   }
   for (const at::Tensor& t : colds) cs.push_back(one_cold(t));
   c10::DeviceGuard guard(like.device());

@@ -251,8 +251,8 @@ class PagePool:
 
     def _emptied(self) -> None:
         """The host's shadow of an empty pool."""
-        self.lens[:] = 0
-        self.hw[:] = 0
+        self.lens.fill(0)
+        self.hw.fill(0)
         self.free_count = self.num_pages
         self.free_exact = True
         self.shared = False
@@ -1464,13 +1464,17 @@ def crop_layers(pools: Sequence[PagePool], batch: int, max_length: int) -> None:
 def reset_layers(pools: Sequence[PagePool]) -> None:
     """``PagePool.reset()`` on every pool, in one launch for a model's GPU pools."""
     pools = list(pools)
-    if len(pools) < 2 or not _one_device(pools):
+    entry = _GROUPS.get(tuple((id(p), p.generation) for p in pools)) if len(pools) > 1 else None
+    if entry is not None and entry["plain"]:  # packed and looked at by an earlier call on these pools
+        _gpu_backend().reset_layers_([entry["group"]], [], pools[0].key_pages)
+    elif len(pools) < 2 or not _one_device(pools):
         for p in pools:
             p.reset()
         return
-    packed = [p._packed() for p in pools]
-    colds = [h[2] for h in packed] if getattr(pools[0], "quantized", False) else []
-    packed[0][3].reset_layers_([h[1] for h in packed], colds, pools[0].key_pages)
+    else:
+        packed = [p._packed() for p in pools]
+        colds = [h[2] for h in packed] if getattr(pools[0], "quantized", False) else []
+        packed[0][3].reset_layers_([h[1] for h in packed], colds, pools[0].key_pages)
     for p in pools:
         p._emptied()
 

@@ -1,4 +1,4 @@
-"""Float64 attention of a drafted tree over a cache: the checker of attend_tree.  Test infrastructure only.
+"""Float64 attention of a drafted tree over a cache: what attend_tree's tests compare with.
 
 A node's positions are gathered one node at a time, so that what it does not see takes no part.  With the
 output come the bounds' ingredients: `weight` = sum of softmax weights times |V| (what relative errors of
