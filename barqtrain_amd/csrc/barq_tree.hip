@@ -37,7 +37,6 @@
 
 #include "barq_kv.h"
 #include "barq_kv_commit.h"
-#include "barq_kv_fp8.h"
 #include "barq_ragged.h"
 #include "fastdiv.h"
 
@@ -626,8 +625,9 @@ __device__ __forceinline__ void lds_only_barrier() { asm volatile("s_waitcnt lgk
 __device__ __forceinline__ float scale_of(uint32_t s) { return __uint_as_float(max(s << 23, 0x00400000u)); }
 
 // Codes 0 and 1 (HIGH: 2 and 3) of four E4M3 codes times a scale, as two 16-bit numbers.  The instruction's products
-// are exact wherever the 16-bit type holds them, and rounded to nearest even elsewhere: equal to dequant2_exact's in
-// all 256 codes at all scale bytes but 255 (compared one by one), E8M0's NaN, which no quantiser stores.
+// are exact wherever the 16-bit type holds them, and rounded to nearest even elsewhere: equal to barq_kv_fp8.h's
+// element by element for all 256 codes at all scale bytes but 255 (compared one by one on the GPU), which is E8M0's
+// NaN and stored by no quantiser.
 template <int E, bool HIGH>
 __device__ __forceinline__ uint32_t scaled2(uint32_t codes, float scale) {
   if constexpr (E == kBF16)
