@@ -331,6 +331,29 @@ def test_fp8_codes_of_every_kind(hip):
     check(pool, q, nk, nv, None, pool.attend_tree(q, nk, nv))
 
 
+@pytest.mark.parametrize("dtype,scales", [(torch.bfloat16, (12, 64, 127, 200, 238)), (torch.float16, (112, 119, 127, 133))])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_fp8_every_code_at_far_scales(hip, dtype, scales, dim):
+    """All codes but NaN's, of values at one scale a call and of keys at a scale a channel, as the gather gives them."""
+    pool = QuantPagePool(max_batch=1, max_blocks=4, page_size=16, kv_heads=2, head_dim=dim, dtype=dtype, device="cuda", window=16)
+    zeros = torch.zeros((1, 2, 48, dim), dtype=dtype, device="cuda")
+    pool.append(zeros, zeros)
+    assert pool.cold_blocks[0] == 2
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda")
+    codes[codes & 127 == 127] = 0
+    q, k, v = nodes_of(pool, 1, 2, 3)
+    for scale in scales:
+        pool.value_scales.fill_(scale)
+        for part in codes.view(-1, dim):
+            pool.value_codes.copy_(part.expand_as(pool.value_codes))
+            check(pool, q * 0, k * 0, v * 0, None, pool.attend_tree(q * 0, k * 0, v * 0))
+    g = torch.Generator().manual_seed(dim)
+    pool.value_scales.fill_(120)
+    pool.key_codes.copy_(codes[torch.randint(0, 256, pool.key_codes.shape, generator=g).cuda()])
+    pool.key_scales.copy_(torch.randint(116, 124, pool.key_scales.shape, generator=g).to(torch.uint8))
+    check(pool, q, k, v, None, pool.attend_tree(q, k, v))
+
+
 def test_single_tokens_agree_with_decode_attention(hip):
     """A chain of T nodes over the cache is decode attention of T tokens after their append."""
     pool = filled([257, 31], dim=128, heads=2, extra=2)
